@@ -215,6 +215,99 @@ MORPHO_API int morpho_sm100_peer_allreduce_finalize(morpho_peer_group_t* group, 
                                                     void* dW_V, void* stream);
 MORPHO_API int morpho_sm100_peer_destroy(morpho_peer_group_t* group);
 
+/* ---- Training-step operators around the attention layer (no reference counterpart: the reference
+ * uses torch's) ----------------------------------------------------------------------------------
+ * Element types of their tensors. */
+#define MORPHO_DTYPE_F16 0
+#define MORPHO_DTYPE_BF16 1
+#define MORPHO_DTYPE_F32 2
+
+/* Layer norm over the last dimension of [rows, dim], optionally of x + residual:
+ *   h = x + residual (in their type; h = x when residual is NULL)
+ *   y = (h - mean(h)) * rstd * weight + bias,   rstd = 1 / sqrt(var(h) + eps)
+ * weight and bias may each be NULL (1 and 0).  Statistics are fp32, as are all sums.  Rows have
+ * unit element stride; a row stride of 0 means dim.  Outputs are contiguous [rows, dim]; mean, rstd
+ * fp32 [rows].  rows may be 0. */
+typedef struct morpho_layer_norm {
+    int64_t rows;
+    int32_t dim;
+    int32_t type;         /* MORPHO_DTYPE_* of x, residual, y, h and their gradients */
+    int32_t weight_type;  /* of weight, bias and their gradients: `type` or MORPHO_DTYPE_F32 */
+    float eps;
+    int64_t stride_x;     /* row strides in elements: x (forward) and h (backward) */
+    int64_t stride_residual;
+    int64_t stride_grad_y;
+    int64_t stride_grad_h;
+} morpho_layer_norm_t;
+
+/* h is written only when residual is given (it may then be x's or residual's own buffer). */
+MORPHO_API int morpho_sm100_layer_norm_forward(const morpho_layer_norm_t* p, const void* x, const void* residual,
+                                               const void* weight, const void* bias, void* y, void* h, float* mean,
+                                               float* rstd, void* stream);
+
+/* Gradient of sum(y * grad_y) + sum(h * grad_h) (grad_h may be NULL): dx, which is the residual's
+ * gradient too, and dweight / dbias (each may be NULL), overwritten.  h, mean and rstd are the
+ * forward's (h = x without a residual).  Sums run in a fixed order: the same bits every run. */
+MORPHO_API size_t morpho_sm100_layer_norm_backward_workspace_size(const morpho_layer_norm_t* p);
+MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_norm_t* p, const void* grad_y, const void* grad_h,
+                                                const void* h, const void* weight, const float* mean,
+                                                const float* rstd, void* dx, void* dweight, void* dbias,
+                                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of z = hidden . weight^T (hidden [tokens, dim], weight [vocab, dim], both fp16
+ * or both bf16, 16-byte aligned) against target (int64 [tokens]), without keeping z:
+ *   lse_t = log sum_v exp z_tv,   loss_t = lse_t - z_t,target(t), 0 where target(t) == ignore_index
+ * loss: fp32 [tokens] (NONE), or one fp32: the sum, or the sum over the number of tokens that are not
+ * ignored (MEAN; 0 if all are).  A target outside [0, vocab) that is not ignore_index makes its
+ * token's lse and loss NaN.  dim must be a multiple of 8, row strides (0 means dim) too.  tokens may be 0. */
+#define MORPHO_REDUCTION_NONE 0
+#define MORPHO_REDUCTION_MEAN 1
+#define MORPHO_REDUCTION_SUM 2
+typedef struct morpho_vocab_loss {
+    int64_t tokens;
+    int32_t vocab;
+    int32_t dim;
+    int32_t type;      /* MORPHO_DTYPE_F16 or MORPHO_DTYPE_BF16 */
+    int32_t reduction; /* MORPHO_REDUCTION_* */
+    int64_t ignore_index;
+    int64_t stride_hidden; /* row strides in elements */
+    int64_t stride_weight;
+} morpho_vocab_loss_t;
+
+MORPHO_API size_t morpho_sm100_linear_cross_entropy_forward_workspace_size(const morpho_vocab_loss_t* p);
+MORPHO_API int morpho_sm100_linear_cross_entropy_forward(const morpho_vocab_loss_t* p, const void* hidden,
+                                                         const void* weight, const int64_t* target, float* loss,
+                                                         float* lse, void* workspace, size_t workspace_bytes,
+                                                         void* stream);
+
+/* dhidden [tokens, dim] and dweight [vocab, dim] (the inputs' type, contiguous, overwritten) for the
+ * loss's gradient grad_loss: fp32 [tokens] (NONE) or one fp32.  The logits are computed again in pieces
+ * of the vocabulary; the workspace holds one piece of their gradient (at most 512 MiB, or 256 columns).
+ * Sums run in a fixed order: the same bits every run. */
+MORPHO_API size_t morpho_sm100_linear_cross_entropy_backward_workspace_size(const morpho_vocab_loss_t* p);
+MORPHO_API int morpho_sm100_linear_cross_entropy_backward(const morpho_vocab_loss_t* p, const float* grad_loss,
+                                                          const void* hidden, const void* weight,
+                                                          const int64_t* target, const float* lse, void* dhidden,
+                                                          void* dweight, void* workspace, size_t workspace_bytes,
+                                                          void* stream);
+
+/* 2-norm over `count` gradients, and clipping by it:
+ *   *norm = sqrt(sum |in|^2) / loss_scale,   out = in * min(1, max_norm / (*norm + 1e-6)) / loss_scale
+ * Each tensor is `count` contiguous elements; out may be in (same type) and must not otherwise overlap
+ * any in.  *norm (fp32, device) is written on the stream: nothing waits on the host. */
+typedef struct morpho_tensor_pair {
+    const void* in;
+    void* out;
+    int64_t count;
+    int32_t in_type;  /* MORPHO_DTYPE_* */
+    int32_t out_type;
+} morpho_tensor_pair_t;
+
+MORPHO_API size_t morpho_sm100_clip_grad_norm_workspace_size(int64_t count);
+MORPHO_API int morpho_sm100_clip_grad_norm(const morpho_tensor_pair_t* pairs, int64_t count, float max_norm,
+                                           float loss_scale, float* norm, void* workspace, size_t workspace_bytes,
+                                           void* stream);
+
 /* Message of the last failure on the calling thread ("" if none). */
 MORPHO_API const char* morpho_sm100_last_error(void);
 

@@ -33,7 +33,8 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
               "--expt-relaxed-constexpr", "-I" + INCLUDE]
-CU_SOURCES = ["host_common.cu", "gemm.cu", "attn_fwd.cu", "attn_bwd.cu", "softmorph.cu", "softmorph_tc.cu", "softmorph_tc_bwd.cu", "pointwise.cu", "capi.cu", "noalloc.cu", "selftest.cu", "score_probe.cu", "peer.cu"]
+CU_SOURCES = ["host_common.cu", "gemm.cu", "attn_fwd.cu", "attn_bwd.cu", "softmorph.cu", "softmorph_tc.cu", "softmorph_tc_bwd.cu", "pointwise.cu", "capi.cu", "noalloc.cu", "selftest.cu", "score_probe.cu", "peer.cu", "layer_norm.cu", "grad_clip.cu", "vocab_loss.cu"]
+SHIM_SOURCES = ["torch_ops.cpp", "torch_train_ops.cpp"]
 
 
 def _headers():
@@ -81,8 +82,8 @@ def build(verbose: bool = False, ptxas_verbose: bool = False, jobs: int | None =
         objs = list(ex.map(lambda s: _compile_cu(s, verbose, ptxas_verbose), srcs))
     if _stale(LIB, objs):
         _run([NVCC] + ARCH + ["-shared", "-o", LIB] + objs, verbose)
-    shim_src = os.path.join(CSRC, "torch_ops.cpp")
-    if _stale(SHIM, [shim_src, LIB] + _headers()):
+    shim_srcs = [os.path.join(CSRC, s) for s in SHIM_SOURCES]
+    if _stale(SHIM, shim_srcs + [LIB] + _headers()):
         incs, libs = _torch_paths()
         import torch
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -90,7 +91,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False, jobs: int | None =
                "-I" + INCLUDE, "-I" + os.path.join(CUDA_HOME, "include"),
                "-I" + sysconfig.get_paths()["include"]]
         cmd += ["-I" + p for p in incs]
-        cmd += [shim_src, "-o", SHIM, "-L" + PKG, "-lmorpho_sm100", "-Wl,-rpath,$ORIGIN"]
+        cmd += shim_srcs + ["-o", SHIM, "-L" + PKG, "-lmorpho_sm100", "-Wl,-rpath,$ORIGIN"]
         for p in libs:
             cmd += ["-L" + p, "-Wl,-rpath," + p]
         cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch"]

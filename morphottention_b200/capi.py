@@ -62,7 +62,19 @@ EXPORTED = (
     "morpho_sm100_peer_bucket",
     "morpho_sm100_peer_allreduce_finalize",
     "morpho_sm100_peer_destroy",
+    "morpho_sm100_layer_norm_forward",
+    "morpho_sm100_layer_norm_backward_workspace_size",
+    "morpho_sm100_layer_norm_backward",
+    "morpho_sm100_linear_cross_entropy_forward_workspace_size",
+    "morpho_sm100_linear_cross_entropy_forward",
+    "morpho_sm100_linear_cross_entropy_backward_workspace_size",
+    "morpho_sm100_linear_cross_entropy_backward",
+    "morpho_sm100_clip_grad_norm_workspace_size",
+    "morpho_sm100_clip_grad_norm",
 )
+MORPHO_DTYPE_F16, MORPHO_DTYPE_BF16, MORPHO_DTYPE_F32 = 0, 1, 2
+MORPHO_REDUCTION_NONE, MORPHO_REDUCTION_MEAN, MORPHO_REDUCTION_SUM = 0, 1, 2
+REDUCTIONS = {"none": MORPHO_REDUCTION_NONE, "mean": MORPHO_REDUCTION_MEAN, "sum": MORPHO_REDUCTION_SUM}
 
 
 class MorphoProblem(ctypes.Structure):
@@ -70,6 +82,24 @@ class MorphoProblem(ctypes.Structure):
                 ("cube_m", ctypes.c_int32), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
                 ("grad_mode", ctypes.c_int32), ("projection", ctypes.c_int32), ("mask_diag", ctypes.c_int32),
                 ("score", ctypes.c_int32), ("tau", ctypes.c_float)]
+
+
+class MorphoLayerNorm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("dim", ctypes.c_int32), ("type", ctypes.c_int32),
+                ("weight_type", ctypes.c_int32), ("eps", ctypes.c_float), ("stride_x", ctypes.c_int64),
+                ("stride_residual", ctypes.c_int64), ("stride_grad_y", ctypes.c_int64),
+                ("stride_grad_h", ctypes.c_int64)]
+
+
+class MorphoVocabLoss(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("vocab", ctypes.c_int32), ("dim", ctypes.c_int32),
+                ("type", ctypes.c_int32), ("reduction", ctypes.c_int32), ("ignore_index", ctypes.c_int64),
+                ("stride_hidden", ctypes.c_int64), ("stride_weight", ctypes.c_int64)]
+
+
+class MorphoTensorPair(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("count", ctypes.c_int64),
+                ("src_type", ctypes.c_int32), ("dst_type", ctypes.c_int32)]
 
 
 class MorphoError(RuntimeError):
@@ -147,6 +177,22 @@ def lib() -> ctypes.CDLL:
     L.morpho_sm100_peer_allreduce_finalize.restype = i32
     L.morpho_sm100_peer_destroy.argtypes = [vp]
     L.morpho_sm100_peer_destroy.restype = i32
+    LN, VL, TP = (ctypes.POINTER(c) for c in (MorphoLayerNorm, MorphoVocabLoss, MorphoTensorPair))
+    L.morpho_sm100_layer_norm_forward.argtypes = [LN] + [vp] * 9
+    L.morpho_sm100_layer_norm_forward.restype = i32
+    L.morpho_sm100_layer_norm_backward_workspace_size.argtypes = [LN]
+    L.morpho_sm100_layer_norm_backward_workspace_size.restype = sz
+    L.morpho_sm100_layer_norm_backward.argtypes = [LN] + [vp] * 10 + [sz, vp]
+    L.morpho_sm100_layer_norm_backward.restype = i32
+    for name, tensors in (("forward", 5), ("backward", 7)):
+        size = getattr(L, f"morpho_sm100_linear_cross_entropy_{name}_workspace_size")
+        size.argtypes, size.restype = [VL], sz
+        fn = getattr(L, f"morpho_sm100_linear_cross_entropy_{name}")
+        fn.argtypes, fn.restype = [VL] + [vp] * (tensors + 1) + [sz, vp], i32
+    L.morpho_sm100_clip_grad_norm_workspace_size.argtypes = [ctypes.c_int64]
+    L.morpho_sm100_clip_grad_norm_workspace_size.restype = sz
+    L.morpho_sm100_clip_grad_norm.argtypes = [TP, ctypes.c_int64, ctypes.c_float, ctypes.c_float, vp, vp, sz, vp]
+    L.morpho_sm100_clip_grad_norm.restype = i32
     _lib = L
     return L
 
