@@ -4,12 +4,11 @@
 //   dz_tv = g_t (exp(z_tv - lse_t) - [v = target(t)]),  dhidden = dz . weight,  dweight = dz^T . hidden
 //
 // Forward: one tcgen05 GEMM whose epilogue reduces each 128-column piece of a logit row in registers to
-// its maximum and its sum of exponentials, so a [T, V] product leaves 16 bytes per row and 256 columns;
+// its maximum and its sum of exponentials, so a [T, V] product leaves 8 bytes per row and 128 columns;
 // a second kernel joins the pieces of a row in a fixed order.
 // Backward: the vocabulary is taken in pieces of columns.  For each piece the logits are computed again
 // (the same GEMM), turned into dz in the epilogue and written as a 16-bit [T, piece] matrix, which two
-// GEMMs read: dhidden += dz . weight_piece (K = piece) and dweight_piece = dz^T . hidden (K = T, in
-// pieces too).
+// GEMMs read: dhidden += dz . weight_piece (K = piece) and dweight_piece = dz^T . hidden (K = T).
 // The arithmetic is 2TVD for the forward and 6TVD for the backward: the tensor cores bound it.
 //
 // dz is rounded to the inputs' type, as tcgen05 needs it, once, and before the common factor of the
@@ -17,8 +16,11 @@
 // that probabilities down to 2^-29 stay normal numbers, and the epilogues multiply the fp32 sums by
 // gmax 2^-15.  (bf16 has fp32's range and takes 2^0.)
 //
-// Warp roles of the GEMMs (320 threads): warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue, as
-// in the projection GEMM.
+// The GEMMs run as 256 x 256 tiles of CTA pairs (cta_group::2): each SM reads half of A's rows and half of
+// B's columns, 32 KB for every 64 of K, where a 128 x 256 tile of one CTA reads 48 KB and leaves its
+// shared memory port busier than its tensor core.  Warp roles (320 threads): warp 0 TMA producer, warp 1
+// MMA issuer (rank 0 of the pair), warps 2-9 epilogue; the accumulator is double-buffered in TMEM, and
+// results leave through TMA stores from a swizzled box per warp.
 #include <algorithm>
 
 #include "elem.cuh"
@@ -29,14 +31,19 @@ namespace morpho {
 namespace {
 
 constexpr uint32_t K_VOCAB = 6;  // kernel id in the device status word
-constexpr int BM = 128, BN = 256, BK = 64;
+constexpr int kTile = 256;       // rows and columns of a CTA pair's tile
+constexpr int kHalf = 128;       // rows of A, columns of B, and rows of the tile that one CTA holds
+constexpr int BK = 64;
 constexpr int kGemmThreads = 320;
-constexpr int kHalf = 128;  // columns an epilogue warp takes
-constexpr int kStages = 4;
-constexpr int kABytes = BM * BK * 2, kBBytes = BN * BK * 2;
-constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kBarOffset = kStages * kStageBytes;
+constexpr int kStages = 3;
+constexpr int kUnits = 2;  // K blocks of 64 in a stage
+constexpr int kOperandBytes = kHalf * BK * 2;
+constexpr int kUnitBytes = 2 * kOperandBytes;
+constexpr int kStageBytes = kUnits * kUnitBytes;
+constexpr int kStoreOffset = kStages * kStageBytes;  // a 4 KB box for each epilogue warp's stores
+constexpr int kBarOffset = kStoreOffset + 8 * 4096;
 constexpr int kSmemBytes = kBarOffset + 256 + 1024;
+static_assert(kSmemBytes <= 232448, "shared memory");
 
 // A target that is neither in [0, vocab) nor ignore_index makes its row's lse NaN.
 struct RowInfo {
@@ -45,10 +52,44 @@ struct RowInfo {
     int vocab;
 };
 
-struct Gemm {
+// What a GEMM's epilogue does with its tile.
+enum Kind : int {
+    kStats,  // row statistics of the logits
+    kDz,     // dz, 16-bit
+    kOut,    // common * sum, 16-bit
+    kPart,   // fp32 partial sums, one slab per K split
+    kPartAdd // the same, added to what is there
+};
+
+// D (M x N) = A (M x K) B (K x N) as 256 x 256 tiles of CTA pairs, K cut into splits.
+struct alignas(64) Task {
+    CUtensorMap a, b, out;
+    int kind;
+    bool a_mn, b_mn;     // stored [K, M] / [K, N] (else [M, K] / [N, K])
+    int a_row0, b_row0;  // first row of A / B in its map
     int M, N;
-    int k_blocks;
-    int tiles_m, tiles_n;
+    int tiles_m, tiles_n, group;  // `group` M tiles share each B tile in L2
+    int k_blocks, kb_per_split;
+    int items_end;  // work items of this task and those before it
+    int v0;         // kDz: the piece's first column of the vocabulary
+};
+
+struct Rowwise {
+    int64_t T;
+    int V;
+    const int64_t* target;
+    float2* part;            // kStats: [ceil(V / 128)][T] maximum and sum of each piece of a row
+    float* zt;               // kStats: [T] logit of the target
+    const float* lse;        // kDz
+    const float* row_scale;  // kDz: r_t 2^15 (0 for ignored rows)
+    const float* common;     // kOut: one value
+};
+
+constexpr int kMaxTasks = 3;
+struct Launch {
+    Task task[kMaxTasks];
+    int tasks;
+    Rowwise rows;
     uint32_t* status;
 };
 
@@ -61,288 +102,380 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return pack_half2(lo, hi);
 }
 
-// ---- epilogues: one thread per row, kHalf columns ---------------------------------------------
+// ---- epilogues: one thread per row, 128 columns at `tacc` ------------------------------------------
+
+// Writes one 4 KB box (32 rows of 128 bytes, this lane's row in `x`) to this warp's staging buffer in the
+// TMA's 128-byte swizzle; lane 0 may then store it.
+__device__ __forceinline__ void stage_box(uint32_t stage, int lane, const uint32_t* x) {
+    if (lane == 0) bulk_wait_read_all();  // the previous box has left
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+        st_shared_u4(stage + lane * 128 + ((g ^ (lane & 7)) << 4), make_uint4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]));
+    fence_proxy_async_smem();
+    __syncwarp();
+}
 
 // Row statistics: the piece's maximum and sum of exp(z - maximum), and the target's logit.
-struct EpiStats {
-    struct Params {
-        int64_t T;
-        int V;
-        const int64_t* target;
-        float2* part;  // [ceil(V / 128)][T]
-        float* zt;     // [T] logit of the target
-    };
-    __device__ static void run(const Params& p, uint32_t tacc, int64_t row, int n0) {
-        const int64_t y = row < p.T ? p.target[row] : -1;
-        float m = -INFINITY, s = 0.f, zt = 0.f;
+template <class Release>
+__device__ __forceinline__ void epi_stats(const Rowwise& p, uint32_t tacc, int64_t row, int n0, Release release) {
+    const int64_t y = row < p.T ? p.target[row] : -1;
+    float m = -INFINITY, s = 0.f, zt = 0.f;
 #pragma unroll 1
-        for (int cc = 0; cc < kHalf; cc += 32) {
-            uint32_t r[32];
-            tmem_ld32(tacc + cc, r);
-            tmem_ld_wait();
-            const int left = p.V - n0 - cc;  // live columns from here on
-            float mx = -INFINITY;
+    for (int cc = 0; cc < kHalf; cc += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld32(tacc + cc, r);
+        tmem_ld_wait();
+        if (cc + 32 == kHalf) release();
+        const int left = p.V - n0 - cc;  // live columns from here on
+        float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (i >= left) r[i] = __float_as_uint(-INFINITY);
-                mx = fmaxf(mx, u2f(r[i]));
-            }
-            const float mn = fmaxf(m, mx);
-            if (mn > -INFINITY) {
-                const float b = mn * kLog2e;
-                float t = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) t += ex2(fmaf(u2f(r[i]), kLog2e, -b));
-                s = s * ex2(fmaf(m, kLog2e, -b)) + t;
-                m = mn;
-            } else {
-                // -inf throughout, or NaN (which a maximum skips)
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (u2f(r[i]) != u2f(r[i])) s = u2f(r[i]);
-            }
-            const int64_t at = y - n0 - cc;
-            if (at >= 0 && at < 32) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i == at) zt = u2f(r[i]);
-            }
+        for (int i = 0; i < 32; ++i) {
+            if (i >= left) r[i] = __float_as_uint(-INFINITY);
+            mx = fmaxf(mx, u2f(r[i]));
         }
-        if (row < p.T) {
-            p.part[static_cast<int64_t>(n0 / kHalf) * p.T + row] = make_float2(m, s);
-            if (y >= n0 && y < n0 + kHalf && y < p.V) p.zt[row] = zt;
+        const float mn = fmaxf(m, mx);
+        if (mn > -INFINITY) {
+            const float b = mn * kLog2e;
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) t += ex2(fmaf(u2f(r[i]), kLog2e, -b));
+            s = s * ex2(fmaf(m, kLog2e, -b)) + t;
+            m = mn;
+        } else {
+            // -inf throughout, or NaN (which a maximum skips)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (u2f(r[i]) != u2f(r[i])) s = u2f(r[i]);
+        }
+        const int64_t at = y - n0 - cc;
+        if (at >= 0 && at < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (i == at) zt = u2f(r[i]);
         }
     }
-};
+    if (row < p.T) {
+        p.part[static_cast<int64_t>(n0 / kHalf) * p.T + row] = make_float2(m, s);
+        if (y >= n0 && y < n0 + kHalf && y < p.V) p.zt[row] = zt;
+    }
+}
 
-// dz of one piece: r_t (exp(z - lse) - [v = target]), 16-bit.
-template <bool BF16>
-struct EpiDz {
-    struct Params {
-        int64_t T;
-        int V, v0, ld;  // vocabulary; the piece's first column; row length of dz
-        const int64_t* target;
-        const float* lse;
-        const float* row_scale;  // r_t 2^15 (0 for ignored rows)
-        uint16_t* dz;            // [T, ld]
-    };
-    __device__ static void run(const Params& p, uint32_t tacc, int64_t row, int n0) {
-        const bool live = row < p.T;
-        const int64_t y = live ? p.target[row] : -1;
-        const float l2 = live ? p.lse[row] * kLog2e : 0.f;
-        const float rs = live ? p.row_scale[row] : 0.f;
+// dz of one piece: r_t (exp(z - lse) - [v = target]).
+template <bool BF16, class Release>
+__device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t tacc, int64_t row, int row0, int n0,
+                                       uint32_t stage, int lane, Release release) {
+    const bool live = row < p.T;
+    const int64_t y = (live ? p.target[row] : -1) - t.v0;
+    const float l2 = live ? p.lse[row] * kLog2e : 0.f;
+    const float rs = live ? p.row_scale[row] : 0.f;
+    const int boxes = min(2, (t.N - n0 + 63) / 64);
 #pragma unroll 1
-        for (int cc = 0; cc < kHalf; cc += 32) {
-            const int c0 = n0 + cc;  // column in the piece
-            if (c0 >= p.ld) break;
+    for (int b = 0; b < boxes; ++b) {
+        uint32_t x[32];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
             uint32_t r[32];
-            tmem_ld32(tacc + cc, r);
+            __syncwarp();
+            tmem_ld32(tacc + b * 64 + q * 32, r);
             tmem_ld_wait();
-            const int64_t at = y - p.v0 - c0;
+            if (q == 1 && b == boxes - 1) release();
             float d[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) d[i] = rs * ex2(fmaf(u2f(r[i]), kLog2e, -l2));
+            const int64_t at = y - (n0 + b * 64 + q * 32);
             if (at >= 0 && at < 32) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     if (i == at) d[i] -= rs;
             }
-            if (rs == 0.f) {  // an ignored row contributes nothing, whatever its logits are
 #pragma unroll
-                for (int i = 0; i < 32; ++i) d[i] = 0.f;
-            }
-            if (live) {
-                uint4* dst = reinterpret_cast<uint4*>(p.dz + row * p.ld + c0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (c0 + 8 * i < p.ld)
-                        dst[i] = make_uint4(pack2<BF16>(d[8 * i], d[8 * i + 1]), pack2<BF16>(d[8 * i + 2], d[8 * i + 3]),
-                                            pack2<BF16>(d[8 * i + 4], d[8 * i + 5]), pack2<BF16>(d[8 * i + 6], d[8 * i + 7]));
+            for (int i = 0; i < 16; ++i) {
+                x[q * 16 + i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
+                if (rs == 0.f) x[q * 16 + i] = 0u;  // an ignored row adds nothing, whatever its logits are
             }
         }
+        stage_box(stage, lane, x);
+        if (lane == 0 && row0 < t.M) {
+            tma_store_2d(&t.out, stage, n0 + b * 64, row0);
+            bulk_commit_group();
+        }
     }
-};
+}
 
-// fp32 running sum over the pieces of K; the last one writes the scaled 16-bit result.
-template <bool BF16>
-struct EpiAcc {
-    struct Params {
-        int64_t M;
-        int N;
-        float* acc;  // [M, N]
-        uint16_t* out;
-        const float* scale;
-        bool first, last;
-    };
-    __device__ static void run(const Params& p, uint32_t tacc, int64_t row, int n0) {
-        const float g = *p.scale;
+// 16-bit result: common * sum.
+template <bool BF16, class Release>
+__device__ __forceinline__ void epi_out(const Rowwise& p, const Task& t, uint32_t tacc, int row0, int n0, uint32_t stage,
+                                        int lane, Release release) {
+    const float g = *p.common;
+    const int boxes = min(2, (t.N - n0 + 63) / 64);
 #pragma unroll 1
-        for (int cc = 0; cc < kHalf; cc += 32) {
-            if (n0 + cc >= p.N) break;
-            uint32_t r[32];
-            tmem_ld32(tacc + cc, r);
-            tmem_ld_wait();
-            if (row < p.M) {
-                float4* acc = reinterpret_cast<float4*>(p.acc + row * p.N + n0 + cc);
-                uint2* dst = reinterpret_cast<uint2*>(p.out + row * p.N + n0 + cc);
+    for (int b = 0; b < boxes; ++b) {
+        uint32_t x[32];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (n0 + cc + 4 * i < p.N) {
-                        float4 x = make_float4(u2f(r[4 * i]), u2f(r[4 * i + 1]), u2f(r[4 * i + 2]), u2f(r[4 * i + 3]));
-                        if (!p.first) {
-                            const float4 o = acc[i];
-                            x.x += o.x;
-                            x.y += o.y;
-                            x.z += o.z;
-                            x.w += o.w;
-                        }
-                        if (p.last)
-                            dst[i] = make_uint2(pack2<BF16>(g * x.x, g * x.y), pack2<BF16>(g * x.z, g * x.w));
-                        else
-                            acc[i] = x;
-                    }
-                }
-            }
+        for (int q = 0; q < 2; ++q) {
+            uint32_t r[32];
+            __syncwarp();
+            tmem_ld32(tacc + b * 64 + q * 32, r);
+            tmem_ld_wait();
+            if (q == 1 && b == boxes - 1) release();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[q * 16 + i] = pack2<BF16>(g * u2f(r[2 * i]), g * u2f(r[2 * i + 1]));
+        }
+        stage_box(stage, lane, x);
+        if (lane == 0 && row0 < t.M) {
+            tma_store_2d(&t.out, stage, n0 + b * 64, row0);
+            bulk_commit_group();
         }
     }
+}
+
+// fp32 partial sums of K split z.
+template <class Release>
+__device__ __forceinline__ void epi_part(const Task& t, uint32_t tacc, int row0, int n0, int z, uint32_t stage, int lane,
+                                         Release release) {
+    const int boxes = min(4, (t.N - n0 + 31) / 32);
+#pragma unroll 1
+    for (int b = 0; b < boxes; ++b) {
+        uint32_t r[32];
+        tmem_ld32(tacc + b * 32, r);
+        tmem_ld_wait();
+        if (b == boxes - 1) release();
+        stage_box(stage, lane, r);
+        if (lane == 0 && row0 < t.M) {
+            if (t.kind == kPartAdd)
+                tma_reduce_add_3d(&t.out, stage, n0 + b * 32, row0, z);
+            else
+                tma_store_3d(&t.out, stage, n0 + b * 32, row0, z);
+            bulk_commit_group();
+        }
+    }
+}
+
+// ---- the GEMM: up to three tasks in one persistent launch of CTA pairs -----------------------------
+
+struct Item {
+    int task, m0, n0, z, kb0, kb1;
 };
 
-// ---- the GEMM -----------------------------------------------------------------------------------
+// Work item w: the tasks one after the other; within a task the splits, then groups of `group` M tiles,
+// then the N tiles, then the M tiles of the group.
+__device__ __forceinline__ Item item_of(const Launch& L, int w) {
+    Item it;
+    int i = 0, start = 0;
+    while (w >= L.task[i].items_end) start = L.task[i++].items_end;
+    const Task& t = L.task[i];
+    int r = w - start;
+    const int mn = t.tiles_m * t.tiles_n;
+    it.task = i;
+    it.z = r / mn;
+    r -= it.z * mn;
+    const int g = r / (t.group * t.tiles_n);
+    r -= g * t.group * t.tiles_n;
+    const int gm = min(t.group, t.tiles_m - g * t.group);
+    const int n = r / gm;
+    it.m0 = (g * t.group + r - n * gm) * kTile;
+    it.n0 = n * kTile;
+    it.kb0 = it.z * t.kb_per_split;
+    it.kb1 = min(t.k_blocks, it.kb0 + t.kb_per_split);
+    return it;
+}
 
-// D (M x N) = A (M x K) B (K x N).  A_MN: A stored [K, M], else [M, K]; B_MN: B stored [K, N], else [N, K].
-template <bool BF16, bool A_MN, bool B_MN, class Epi>
-__global__ void __launch_bounds__(kGemmThreads, 1)
-    vocab_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const int a_row0,
-                      const int b_row0, const Gemm args, const typename Epi::Params ep) {
+template <bool BF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) vocab_gemm_kernel(const __grid_constant__ Launch L) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOffset);
     constexpr int NB = 2 * kStages + 5;  // full, empty, acc_full[2], acc_empty[2], drain
+    static_assert(NB * 8 + 8 <= 256, "barrier block");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     const int warp = warp_id();
     const int lane = threadIdx.x & 31;
-    const int n_items = args.tiles_m * args.tiles_n;
+    const int rank = static_cast<int>(cluster_rank());
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int n_items = L.task[L.tasks - 1].items_end;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kStages);
     const uint32_t acc_full0 = smem_u32(bars + 2 * kStages), acc_empty0 = smem_u32(bars + 2 * kStages + 2);
     const uint32_t drain_bar = smem_u32(bars + 2 * kStages + 4);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 1);
+            mbar_init(full0 + 8 * s, 1);   // used in rank 0: its producer's arrival and both CTAs' bytes
+            mbar_init(empty0 + 8 * s, 1);  // rank 0's commit, to both
         }
         for (int a = 0; a < 2; ++a) {
-            mbar_init(acc_full0 + 8 * a, 1);
-            mbar_init(acc_empty0 + 8 * a, 8);
+            mbar_init(acc_full0 + 8 * a, 1);    // rank 0's commit, to both
+            mbar_init(acc_empty0 + 8 * a, 16);  // used in rank 0: the epilogue warps of both
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
         fence_barrier_init();
-        tma_prefetch_desc(&tmA);
-        tma_prefetch_desc(&tmB);
+        for (int i = 0; i < L.tasks; ++i) {
+            tma_prefetch_desc(&L.task[i].a);
+            tma_prefetch_desc(&L.task[i].b);
+        }
     }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), 2 * BN);
-        tmem_relinquish();
-    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), 2 * kTile);
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
+        // ---------------- TMA producer, in both CTAs ----------------
         if (lane == 0) {
             int g = 0;
-            for (int w = blockIdx.x; w < n_items && !*abort_flag; w += gridDim.x) {
-                const int m0 = (w / args.tiles_n) * BM, n0 = (w % args.tiles_n) * BN;
-                for (int kb = 0; kb < args.k_blocks; ++kb, ++g) {
+            for (int w = first; w < n_items && !*abort_flag; w += step) {
+                const Item it = item_of(L, w);
+                const Task& t = L.task[it.task];
+                const int m = it.m0 + rank * kHalf, n = it.n0 + rank * kHalf;
+                for (int kb = it.kb0; kb < it.kb1; kb += kUnits, ++g) {
                     const int s = g % kStages;
-                    if (g >= kStages && !mbar_wait(empty0 + 8 * s, ((g / kStages) & 1) ^ 1, args.status, K_VOCAB, 1)) {
+                    if (g >= kStages && !mbar_wait(empty0 + 8 * s, ((g / kStages) & 1) ^ 1, L.status, K_VOCAB, 1)) {
                         *abort_flag = 1u;
                         break;
                     }
-                    const uint32_t sA = smem_u32(smem + s * kStageBytes), sB = sA + kABytes, fb = full0 + 8 * s;
-                    const int k0 = kb * BK;
-                    mbar_arrive_expect_tx(fb, kStageBytes);
-                    if (A_MN) {
-                        tma_load_2d(sA, &tmA, fb, m0, a_row0 + k0);
-                        tma_load_2d(sA + 64 * 128, &tmA, fb, m0 + 64, a_row0 + k0);
-                    } else {
-                        tma_load_2d(sA, &tmA, fb, k0, a_row0 + m0);
-                    }
-                    if (B_MN) {
-#pragma unroll
-                        for (int c = 0; c < BN / 64; ++c) tma_load_2d(sB + c * 64 * 128, &tmB, fb, n0 + 64 * c, b_row0 + k0);
-                    } else {
-                        tma_load_2d(sB, &tmB, fb, k0, b_row0 + n0);
+                    const uint32_t fb = cluster_addr(full0 + 8 * s, 0);
+                    const int units = min(kUnits, it.kb1 - kb);
+                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, units * 2 * kUnitBytes);
+                    for (int u = 0; u < units; ++u) {
+                        const uint32_t sA = smem_u32(smem + s * kStageBytes + u * kUnitBytes), sB = sA + kOperandBytes;
+                        const int k0 = (kb + u) * BK;
+                        if (t.a_mn) {
+                            tma_load_2d_pair(sA, &t.a, fb, m, t.a_row0 + k0);
+                            tma_load_2d_pair(sA + 64 * 128, &t.a, fb, m + 64, t.a_row0 + k0);
+                        } else {
+                            tma_load_2d_pair(sA, &t.a, fb, k0, t.a_row0 + m);
+                        }
+                        if (t.b_mn) {
+                            tma_load_2d_pair(sB, &t.b, fb, n, t.b_row0 + k0);
+                            tma_load_2d_pair(sB + 64 * 128, &t.b, fb, n + 64, t.b_row0 + k0);
+                        } else {
+                            tma_load_2d_pair(sB, &t.b, fb, k0, t.b_row0 + n);
+                        }
                     }
                 }
             }
-            if (*abort_flag)
+            // No CTA leaves while commits to its barriers are on their way.
+            for (int i = max(0, g - kStages); i < g && !*abort_flag; ++i)
+                mbar_wait(empty0 + 8 * (i % kStages), (i / kStages) & 1, L.status, K_VOCAB, 7);
+            // Drain: the loads of both CTAs complete on rank 0's barriers; rank 1 stays until the
+            // cluster barrier at the end.
+            if (*abort_flag && rank == 0)
                 for (int i = max(0, g - kStages); i < g; ++i)
-                    mbar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, args.status, K_VOCAB, 2);
+                    mbar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, L.status, K_VOCAB, 2);
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc = make_idesc_f16(BM, BN, A_MN, B_MN) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
-        bool ok = true;
-        int g = 0, j = 0;
-        for (int w = blockIdx.x; ok && w < n_items; w += gridDim.x, ++j) {
-            const int a = j & 1;
-            if (j >= 2 && !mbar_wait_warp(acc_empty0 + 8 * a, ((j >> 1) & 1) ^ 1, args.status, K_VOCAB, 6)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
-            const uint32_t dacc = tmem + a * BN;
-            for (int i = 0; i < args.k_blocks; ++i, ++g) {
-                const int s = g % kStages;
-                if (!mbar_wait_warp(full0 + 8 * s, (g / kStages) & 1, args.status, K_VOCAB, 3)) {
+        // ---------------- MMA issuer, one thread of rank 0 ----------------
+        if (rank == 0 && lane == 0) {
+            constexpr uint32_t type_bits = BF16 ? (1u << 7) | (1u << 10) : 0u;
+            bool ok = true;
+            int g = 0, j = 0;
+            for (int w = first; ok && w < n_items; w += step, ++j) {
+                const Item it = item_of(L, w);
+                const bool a_mn = L.task[it.task].a_mn, b_mn = L.task[it.task].b_mn;
+                const uint32_t idesc = make_idesc_f16(kTile, kTile, a_mn, b_mn) | type_bits;
+                // K-major: 8-row groups of 1 KB, K = 16 every 32 bytes; MN-major: 64-column groups of
+                // 8 KB, 8-row groups of 1 KB, K = 16 every 2 KB
+                const uint32_t a_lbo = a_mn ? 64 * 128 : 16, b_lbo = b_mn ? 64 * 128 : 16;
+                const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+                const int a = j & 1;
+                if (j >= 2 && !mbar_wait_cluster(acc_empty0 + 8 * a, ((j >> 1) & 1) ^ 1, L.status, K_VOCAB, 6)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t sA = smem_u32(smem + s * kStageBytes), sB = sA + kABytes;
+                const uint32_t dacc = tmem + a * kTile;
+                for (int i = it.kb0; i < it.kb1; i += kUnits, ++g) {
+                    const int s = g % kStages;
+                    // (what the TMA wrote needs no tcgen05 fence: the MMAs read it through the async proxy)
+                    if (!mbar_wait(full0 + 8 * s, (g / kStages) & 1, L.status, K_VOCAB, 3)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sA = smem_u32(smem + s * kStageBytes);
 #pragma unroll
-                for (int ks = 0; ks < BK / 16; ++ks) {
-                    const uint64_t ad = A_MN ? make_sdesc(sA + ks * 2048, 64 * 128, 1024, SW_128) : make_sdesc(sA + ks * 32, 16, 1024, SW_128);
-                    const uint64_t bd = B_MN ? make_sdesc(sB + ks * 2048, 64 * 128, 1024, SW_128) : make_sdesc(sB + ks * 32, 16, 1024, SW_128);
-                    umma_ss_w(dacc, ad, bd, idesc, (i > 0 || ks > 0) ? 1u : 0u);
+                    for (int u = 0; u < kUnits; ++u) {
+                        if (u == 0 || i + u < it.kb1) {
+#pragma unroll
+                            for (int ks = 0; ks < BK / 16; ++ks)
+                                umma_ss_pair(dacc, make_sdesc(sA + u * kUnitBytes + ks * a_step, a_lbo, 1024, SW_128),
+                                               make_sdesc(sA + u * kUnitBytes + kOperandBytes + ks * b_step, b_lbo, 1024, SW_128), idesc,
+                                               (i > it.kb0 || u > 0 || ks > 0) ? 1u : 0u);
+                        }
+                    }
+                    umma_commit_pair(empty0 + 8 * s);
                 }
-                umma_commit_w(empty0 + 8 * s);
+                if (ok) umma_commit_pair(acc_full0 + 8 * a);
             }
-            if (ok) umma_commit_w(acc_full0 + 8 * a);
-        }
-        if (!ok) {
-            *abort_flag = 1u;
-            umma_commit_w(drain_bar);
-            mbar_wait_warp(drain_bar, 0, args.status, K_VOCAB, 4);
-            umma_commit_w(acc_full0);
-            umma_commit_w(acc_full0 + 8);
+            if (!ok) {
+                *abort_flag = 1u;
+                umma_commit_pair(drain_bar);
+                mbar_wait(drain_bar, 0, L.status, K_VOCAB, 4);
+                umma_commit_pair(acc_full0);
+                umma_commit_pair(acc_full0 + 8);
+            }
         }
     } else {
+        // ---------------- epilogue, in both CTAs ----------------
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+        const uint32_t stage = smem_u32(smem + kStoreOffset + (warp - 2) * 4096);
         int j = 0;
-        for (int w = blockIdx.x; w < n_items; w += gridDim.x, ++j) {
-            const int m0 = (w / args.tiles_n) * BM, n0 = (w % args.tiles_n) * BN;
+        for (int w = first; w < n_items; w += step, ++j) {
+            const Item it = item_of(L, w);
+            const Task& t = L.task[it.task];
             const int a = j & 1;
-            if (!mbar_wait_warp(acc_full0 + 8 * a, (j >> 1) & 1, args.status, K_VOCAB, 5) || *abort_flag) {
+            if (!mbar_wait_warp(acc_full0 + 8 * a, (j >> 1) & 1, L.status, K_VOCAB, 5) || *abort_flag) {
                 *abort_flag = 1u;
                 break;
             }
             tc_fence_after();
-            if (n0 + half * kHalf < args.N)
-                Epi::run(ep, tmem + a * BN + half * kHalf + lane_off, static_cast<int64_t>(m0) + quad * 32 + lane, n0 + half * kHalf);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty0 + 8 * a);
+            const int row0 = it.m0 + rank * kHalf + quad * 32, n0 = it.n0 + half * kHalf;
+            const uint32_t tacc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + a * kTile + half * kHalf;
+            auto release = [&]() {  // this warp has read its part of the accumulator
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * a, 0));
+            };
+            if (n0 >= t.N) {
+                release();
+            } else if (t.kind == kStats) {
+                epi_stats(L.rows, tacc, static_cast<int64_t>(row0) + lane, n0, release);
+            } else if (t.kind == kDz) {
+                epi_dz<BF16>(L.rows, t, tacc, static_cast<int64_t>(row0) + lane, row0, n0, stage, lane, release);
+            } else if (t.kind == kOut) {
+                epi_out<BF16>(L.rows, t, tacc, row0, n0, stage, lane, release);
+            } else {
+                epi_part(t, tacc, row0, n0, it.z, stage, lane, release);
+            }
         }
+        if (lane == 0) bulk_wait_all();  // the stores have read this CTA's shared memory and are done
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        tmem_dealloc_pair(tmem, 2 * kTile);
+    }
+}
+
+// out = common * sum of the partial slabs (in their order): 16-bit, eight elements a thread.
+template <bool BF16>
+__global__ void __launch_bounds__(256) vocab_finish_kernel(const float* part, int slabs, int64_t elems, const float* common,
+                                                           uint16_t* out) {
+    const float g = *common;
+    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < elems; i += static_cast<int64_t>(gridDim.x) * 2048) {
+        float4 a = *reinterpret_cast<const float4*>(part + i), b = *reinterpret_cast<const float4*>(part + i + 4);
+        for (int s = 1; s < slabs; ++s) {
+            const float4 c = *reinterpret_cast<const float4*>(part + s * elems + i), d = *reinterpret_cast<const float4*>(part + s * elems + i + 4);
+            a.x += c.x, a.y += c.y, a.z += c.z, a.w += c.w;
+            b.x += d.x, b.y += d.y, b.z += d.z, b.w += d.w;
+        }
+        *reinterpret_cast<uint4*>(out + i) = make_uint4(pack2<BF16>(g * a.x, g * a.y), pack2<BF16>(g * a.z, g * a.w),
+                                                        pack2<BF16>(g * b.x, g * b.y), pack2<BF16>(g * b.z, g * b.w));
     }
 }
 
@@ -440,7 +573,7 @@ __global__ void __launch_bounds__(1024) vocab_scale_kernel(const float* grad, in
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr size_t kPieceBytes = 512u << 20;  // dz of one piece of the vocabulary, at most
+constexpr size_t kPieceBytes = 256u << 20;  // dz of one piece of the vocabulary, at most; two are held
 // Terms of one tensor-core sum, at most.  The tensor core truncates its fp32 accumulator at every
 // K = 16 step, which biases a long sum towards zero (2.3e-8 of it a step; 1.2 % measured after 2^23
 // terms), so longer sums are joined from sums of this length by rounded fp32 additions.
@@ -465,12 +598,38 @@ int validate_loss(const morpho_vocab_loss_t* p) {
 int64_t ld_hidden(const morpho_vocab_loss_t* p) { return p->stride_hidden ? p->stride_hidden : p->dim; }
 int64_t ld_weight(const morpho_vocab_loss_t* p) { return p->stride_weight ? p->stride_weight : p->dim; }
 
-// Columns of a vocabulary piece, a multiple of the tile width: as many as dz's limit and the length of a
-// tensor-core sum allow.
-int piece_cols(const morpho_vocab_loss_t* p) {
-    const int64_t fit = static_cast<int64_t>(kPieceBytes / 2 / std::max<int64_t>(1, p->tokens)) / BN * BN;
-    const int64_t all = (p->vocab + BN - 1) / BN * static_cast<int64_t>(BN);
-    return static_cast<int>(std::min<int64_t>({all, std::max<int64_t>(BN, fit), kMaxK}));
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How the backward is cut: columns of a vocabulary piece (a multiple of the tile), and K splits of the
+// dhidden (K = piece) and dweight (K = tokens) GEMMs.
+struct Cut {
+    int cols, pieces, splits_h, splits_w;
+};
+
+// K splits of a GEMM of `tiles` tiles and `kb` K blocks in a launch with `total` tile * K-block units on
+// `pairs` CTA pairs: no split longer than kMaxK, nor than a third of a pair's share of the launch (so that
+// uneven shares cost little), nor, for the latter, shorter than 32 blocks (a partial tile costs about as
+// much to write and join as 16 blocks to compute).
+int splits_of(int64_t kb, int64_t total, int pairs) {
+    const int64_t share = std::max<int64_t>(32, total / (3 * pairs));
+    const int64_t splits = ceil_div(kb, std::min<int64_t>(share, kMaxK / BK));
+    const int64_t per = ceil_div(kb, splits);
+    return static_cast<int>(ceil_div(kb, per));  // no empty split
+}
+
+Cut cut_of(const morpho_vocab_loss_t* p, int sms) {
+    Cut c;
+    const int64_t T = std::max<int64_t>(1, p->tokens);
+    const int64_t all = ceil_div(p->vocab, kTile) * kTile;
+    const int64_t fit = static_cast<int64_t>(kPieceBytes / 2) / T / kTile * kTile;
+    c.cols = static_cast<int>(std::min(all, std::max<int64_t>(kTile, fit)));
+    c.pieces = static_cast<int>(ceil_div(p->vocab, c.cols));
+    const int64_t tt = ceil_div(T, kTile), tv = c.cols / kTile, td = ceil_div(p->dim, kTile);
+    const int64_t total = tt * tv * ceil_div(p->dim, BK) + tt * td * (c.cols / BK) + tv * td * ceil_div(T, BK);
+    const int pairs = std::max(1, sms / 2);
+    c.splits_h = splits_of(ceil_div(std::min<int64_t>(c.cols, p->vocab), BK), total, pairs);
+    c.splits_w = splits_of(ceil_div(T, BK), total, pairs);
+    return c;
 }
 
 struct Bump {
@@ -497,47 +656,99 @@ void plan_forward(Bump& b, const morpho_vocab_loss_t* p, FwdPlan* f) {
 }
 
 struct BwdPlan {
-    int cols;
-    uint16_t* dz;
-    float *row_scale, *common, *acc, *wacc;
+    Cut cut;
+    uint16_t* dz[2];
+    float *row_scale, *common, *hpart, *wpart;
 };
-void plan_backward(Bump& b, const morpho_vocab_loss_t* p, BwdPlan* f) {
-    f->cols = piece_cols(p);
-    f->dz = b.take<uint16_t>(static_cast<size_t>(p->tokens) * f->cols);
-    f->row_scale = b.take<float>(p->tokens);
+void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
+    f->cut = cut_of(p, sms);
+    const Cut& c = f->cut;
+    const size_t T = p->tokens, D = p->dim;
+    for (int i = 0; i < 2; ++i) f->dz[i] = b.take<uint16_t>(i < c.pieces ? T * c.cols : 0);
+    f->row_scale = b.take<float>(T);
     f->common = b.take<float>(64);
-    f->acc = b.take<float>(f->cols < p->vocab ? static_cast<size_t>(p->tokens) * p->dim : 0);
-    f->wacc = b.take<float>(p->tokens > kMaxK ? static_cast<size_t>(f->cols) * p->dim : 0);
+    f->hpart = b.take<float>(c.pieces > 1 || c.splits_h > 1 ? c.splits_h * T * D : 0);
+    f->wpart = b.take<float>(c.splits_w > 1 ? static_cast<size_t>(c.splits_w) * c.cols * D : 0);
 }
 
-template <bool BF16, bool A_MN, bool B_MN, class Epi>
-int run(const DeviceInfo& dev, const CUtensorMap& tA, const CUtensorMap& tB, int a_row0, int b_row0, int64_t M, int N, int64_t K,
-        const typename Epi::Params& ep, cudaStream_t stream, const char* name) {
-    auto kern = vocab_gemm_kernel<BF16, A_MN, B_MN, Epi>;
+int sm_count() {
+    DeviceInfo dev;
+    const int sms = current_device_info(&dev) == MORPHO_OK ? dev.sms : 148;
+    clear_error();
+    return sms;
+}
+
+// A 16-bit [rows, cols] matrix for loads of 128 rows x 64 K (K-major), or of 64 K x 64 columns (MN-major).
+int load_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn) {
+    return make_tmap_2d_f16(m, base, rows, cols, ld, mn ? BK : kHalf, BK);
+}
+// Stores of 32 rows x 128 bytes: a 16-bit matrix, and fp32 slabs [slabs, rows, cols].
+int store_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+    return make_tmap_2d_f16(m, base, rows, cols, ld, 32, 64);
+}
+int slab_map(CUtensorMap* m, const void* base, int64_t slabs, int64_t rows, int64_t cols) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), static_cast<uint64_t>(slabs)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(cols) * 4, static_cast<uint64_t>(rows) * cols * 4};
+    const uint32_t box[3] = {32, 32, 1};
+    return make_tmap(m, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Appends a task whose maps are set.
+int add_task(Launch* L, Task& t, int kind, bool a_mn, bool b_mn, int64_t M, int64_t N, int64_t K, int splits) {
+    t.kind = kind;
+    t.a_mn = a_mn;
+    t.b_mn = b_mn;
+    t.M = static_cast<int>(M);
+    t.N = static_cast<int>(N);
+    t.tiles_m = static_cast<int>(ceil_div(M, kTile));
+    t.tiles_n = static_cast<int>(ceil_div(N, kTile));
+    // 8 M tiles x about 9 N tiles at a time on 74 CTA pairs; a few N tiles run side by side
+    t.group = t.tiles_n <= 8 ? 1 : 8;
+    t.k_blocks = static_cast<int>(ceil_div(K, BK));
+    t.kb_per_split = static_cast<int>(ceil_div(t.k_blocks, splits));
+    const int64_t before = L->tasks > 0 ? L->task[L->tasks - 1].items_end : 0;
+    const int64_t end = before + static_cast<int64_t>(t.tiles_m) * t.tiles_n * ceil_div(t.k_blocks, t.kb_per_split);
+    if (end > 2147483647LL - 65536) return set_error(MORPHO_ERR_INVALID, "cross entropy: too many tiles");
+    t.items_end = static_cast<int>(end);
+    L->task[L->tasks++] = t;
+    return MORPHO_OK;
+}
+
+template <bool BF16>
+int launch(const DeviceInfo& dev, Launch& L, cudaStream_t stream, const char* name) {
+    auto kern = vocab_gemm_kernel<BF16>;
     MORPHO_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-    Gemm g;
-    g.M = static_cast<int>(M);
-    g.N = N;
-    g.k_blocks = static_cast<int>((K + BK - 1) / BK);
-    g.tiles_m = static_cast<int>((M + BM - 1) / BM);
-    g.tiles_n = (N + BN - 1) / BN;
-    g.status = dev.status;
-    const int64_t items = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    if (items > 2147483647LL) return set_error(MORPHO_ERR_INVALID, "cross entropy: too many tiles");
+    L.status = dev.status;
+    const int pairs = std::min(L.task[L.tasks - 1].items_end, std::max(1, dev.sms / 2));
     prof_begin(stream, name);
-    kern<<<static_cast<unsigned>(std::min<int64_t>(items, dev.sms)), kGemmThreads, kSmemBytes, stream>>>(tA, tB, a_row0, b_row0, g, ep);
+    kern<<<2 * pairs, kGemmThreads, kSmemBytes, stream>>>(L);
     MORPHO_LAUNCH_CHECK(name);
+    return MORPHO_OK;
+}
+
+template <bool BF16>
+int finish(const DeviceInfo& dev, const float* part, int slabs, int64_t elems, const float* common, void* out, cudaStream_t stream) {
+    prof_begin(stream, "vocab_finish");
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 2048), 8 * dev.sms));
+    vocab_finish_kernel<BF16><<<grid, 256, 0, stream>>>(part, slabs, elems, common, static_cast<uint16_t*>(out));
+    MORPHO_LAUNCH_CHECK("vocab_finish");
     return MORPHO_OK;
 }
 
 template <bool BF16>
 int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* hidden, const void* weight,
               const RowInfo& info, float* loss, float* lse, const FwdPlan& f, cudaStream_t stream) {
-    CUtensorMap tA, tB;
-    MORPHO_TRY(make_tmap_2d_f16(&tA, hidden, p->tokens, p->dim, ld_hidden(p), BM, BK));
-    MORPHO_TRY(make_tmap_2d_f16(&tB, weight, p->vocab, p->dim, ld_weight(p), BN, BK));
-    EpiStats::Params ep{p->tokens, p->vocab, info.target, f.part, f.zt};
-    MORPHO_TRY((run<BF16, false, false, EpiStats>(dev, tA, tB, 0, 0, p->tokens, p->vocab, p->dim, ep, stream, "vocab_stats")));
+    Launch L{};
+    L.rows.T = p->tokens;
+    L.rows.V = p->vocab;
+    L.rows.target = info.target;
+    L.rows.part = f.part;
+    L.rows.zt = f.zt;
+    Task t{};
+    MORPHO_TRY(load_map(&t.a, hidden, p->tokens, p->dim, ld_hidden(p), false));
+    MORPHO_TRY(load_map(&t.b, weight, p->vocab, p->dim, ld_weight(p), false));
+    MORPHO_TRY(add_task(&L, t, kStats, false, false, p->tokens, p->vocab, p->dim, 1));
+    MORPHO_TRY(launch<BF16>(dev, L, stream, "vocab_stats"));
     const bool none = p->reduction == MORPHO_REDUCTION_NONE;
     prof_begin(stream, "vocab_join");
     vocab_join_kernel<<<static_cast<unsigned>((p->tokens + 31) / 32), 256, 0, stream>>>(
@@ -551,33 +762,64 @@ int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* h
     return MORPHO_OK;
 }
 
+// One launch computes dz of piece i + 1 beside the two products that read dz of piece i (the two dz
+// buffers alternate), so the tiles of all three fill the SMs together.
 template <bool BF16>
 int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float* grad, const void* hidden, const void* weight,
                const RowInfo& info, const float* lse, void* dhidden, void* dweight, const BwdPlan& f, cudaStream_t stream) {
     prof_begin(stream, "vocab_scale");
     vocab_scale_kernel<<<1, 1024, 0, stream>>>(grad, p->tokens, info, p->reduction, BF16 ? 1.0f : 32768.0f, f.row_scale, f.common);
     MORPHO_LAUNCH_CHECK("vocab_scale");
-    CUtensorMap tH, tW, tDz, tWn, tDzT, tHn;
-    MORPHO_TRY(make_tmap_2d_f16(&tH, hidden, p->tokens, p->dim, ld_hidden(p), BM, BK));
-    MORPHO_TRY(make_tmap_2d_f16(&tW, weight, p->vocab, p->dim, ld_weight(p), BN, BK));
-    MORPHO_TRY(make_tmap_2d_f16(&tWn, weight, p->vocab, p->dim, ld_weight(p), BK, 64));
-    MORPHO_TRY(make_tmap_2d_f16(&tHn, hidden, p->tokens, p->dim, ld_hidden(p), BK, 64));
-    for (int v0 = 0; v0 < p->vocab; v0 += f.cols) {
-        const int n = std::min(f.cols, p->vocab - v0);
-        MORPHO_TRY(make_tmap_2d_f16(&tDz, f.dz, p->tokens, n, f.cols, BM, BK));
-        MORPHO_TRY(make_tmap_2d_f16(&tDzT, f.dz, p->tokens, n, f.cols, BK, 64));
-        typename EpiDz<BF16>::Params ez{p->tokens, p->vocab, v0, f.cols, info.target, lse, f.row_scale, f.dz};
-        MORPHO_TRY((run<BF16, false, false, EpiDz<BF16>>(dev, tH, tW, 0, v0, p->tokens, n, p->dim, ez, stream, "vocab_dz")));
-        typename EpiAcc<BF16>::Params ea{p->tokens, p->dim, f.acc, static_cast<uint16_t*>(dhidden), f.common, v0 == 0, v0 + n >= p->vocab};
-        MORPHO_TRY((run<BF16, false, true, EpiAcc<BF16>>(dev, tDz, tWn, 0, v0, p->tokens, p->dim, n, ea, stream, "vocab_dhidden")));
-        for (int64_t t0 = 0; t0 < p->tokens; t0 += kMaxK) {
-            const int64_t k = std::min<int64_t>(kMaxK, p->tokens - t0);
-            typename EpiAcc<BF16>::Params ew{n, p->dim, f.wacc, static_cast<uint16_t*>(dweight) + static_cast<int64_t>(v0) * p->dim,
-                                             f.common, t0 == 0, t0 + k >= p->tokens};
-            MORPHO_TRY((run<BF16, true, true, EpiAcc<BF16>>(dev, tDzT, tHn, static_cast<int>(t0), static_cast<int>(t0), n, p->dim, k, ew,
-                                                            stream, "vocab_dweight")));
+    const Cut& c = f.cut;
+    const int64_t T = p->tokens, D = p->dim;
+    auto width = [&](int i) { return std::min<int64_t>(c.cols, p->vocab - static_cast<int64_t>(i) * c.cols); };
+    for (int i = -1; i < c.pieces; ++i) {
+        Launch L{};
+        L.rows.T = T;
+        L.rows.V = p->vocab;
+        L.rows.target = info.target;
+        L.rows.lse = lse;
+        L.rows.row_scale = f.row_scale;
+        L.rows.common = f.common;
+        if (i >= 0) {
+            const int v0 = i * c.cols;
+            const int64_t n = width(i);
+            Task w{}, h{};
+            uint16_t* dw = static_cast<uint16_t*>(dweight) + static_cast<int64_t>(v0) * D;
+            MORPHO_TRY(load_map(&w.a, f.dz[i & 1], T, n, c.cols, true));
+            MORPHO_TRY(load_map(&w.b, hidden, T, D, ld_hidden(p), true));
+            if (c.splits_w > 1)
+                MORPHO_TRY(slab_map(&w.out, f.wpart, c.splits_w, n, D));
+            else
+                MORPHO_TRY(store_map(&w.out, dw, n, D, D));
+            MORPHO_TRY(add_task(&L, w, c.splits_w > 1 ? kPart : kOut, true, true, n, D, T, c.splits_w));
+            MORPHO_TRY(load_map(&h.a, f.dz[i & 1], T, n, c.cols, false));
+            MORPHO_TRY(load_map(&h.b, weight, p->vocab, D, ld_weight(p), true));
+            h.b_row0 = v0;
+            const bool direct = c.pieces == 1 && c.splits_h == 1;
+            // a shorter last piece may need fewer splits: their slabs keep the earlier pieces' sums
+            if (direct)
+                MORPHO_TRY(store_map(&h.out, dhidden, T, D, D));
+            else
+                MORPHO_TRY(slab_map(&h.out, f.hpart, c.splits_h, T, D));
+            MORPHO_TRY(add_task(&L, h, direct ? kOut : i == 0 ? kPart : kPartAdd, false, true, T, D, n,
+                                static_cast<int>(std::min<int64_t>(c.splits_h, ceil_div(n, BK)))));
         }
+        if (i + 1 < c.pieces) {
+            Task z{};
+            z.v0 = (i + 1) * c.cols;
+            z.b_row0 = z.v0;
+            MORPHO_TRY(load_map(&z.a, hidden, T, D, ld_hidden(p), false));
+            MORPHO_TRY(load_map(&z.b, weight, p->vocab, D, ld_weight(p), false));
+            MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, width(i + 1), c.cols));
+            MORPHO_TRY(add_task(&L, z, kDz, false, false, T, width(i + 1), D, 1));
+        }
+        MORPHO_TRY(launch<BF16>(dev, L, stream, i < 0 ? "vocab_dz" : "vocab_grad"));
+        if (i >= 0 && c.splits_w > 1)
+            MORPHO_TRY(finish<BF16>(dev, f.wpart, c.splits_w, width(i) * D, f.common,
+                                    static_cast<uint16_t*>(dweight) + static_cast<int64_t>(i) * c.cols * D, stream));
     }
+    if (c.pieces > 1 || c.splits_h > 1) MORPHO_TRY(finish<BF16>(dev, f.hpart, c.splits_h, T * D, f.common, dhidden, stream));
     return MORPHO_OK;
 }
 
@@ -606,7 +848,7 @@ extern "C" MORPHO_API size_t morpho_sm100_linear_cross_entropy_backward_workspac
     if (validate_loss(p) != MORPHO_OK) return 0;
     Bump b{nullptr};
     BwdPlan f;
-    plan_backward(b, p, &f);
+    plan_backward(b, p, sm_count(), &f);
     return b.off + 256;
 }
 
@@ -665,7 +907,7 @@ extern "C" MORPHO_API int morpho_sm100_linear_cross_entropy_backward(const morph
     MORPHO_TRY(current_device_info(&dev));
     Bump b{static_cast<uint8_t*>(workspace)};
     BwdPlan f;
-    plan_backward(b, p, &f);
+    plan_backward(b, p, dev.sms, &f);
     const RowInfo info{target, p->ignore_index, p->vocab};
     return p->type == MORPHO_DTYPE_BF16 ? backward_t<true>(dev, p, grad_loss, hidden, weight, info, lse, dhidden, dweight, f, st)
                                         : backward_t<false>(dev, p, grad_loss, hidden, weight, info, lse, dhidden, dweight, f, st);
