@@ -10,6 +10,12 @@
 
 namespace morpho {
 
+// Wait until the kernels before this one on the stream have ended and their writes are visible; every
+// CTA of a kernel launched by launch_after calls it before it touches global memory.  And let the next
+// such kernel be set up from here on.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -57,6 +57,23 @@ int prof_collect(char* names, int name_len, float* total_ms, int* counts, int ma
         ::morpho::prof_end(name, stream);                                                                      \
     } while (0)
 
+// Launch a kernel that begins with pdl_wait(): its CTAs may be set up while the kernel before it on the
+// stream drains (programmatic stream serialization), instead of after it has ended.
+template <class... P, class... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Tiled tensor map over a row-major fp16/fp32 tensor.  dims/box are innermost first;
 // row_strides_bytes has rank-1 entries (stride of dims[1], dims[2], ...).
 int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank, const uint64_t* dims,

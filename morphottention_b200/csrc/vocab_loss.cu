@@ -45,13 +45,6 @@ constexpr int kBarOffset = kStoreOffset + 8 * 4096;
 constexpr int kSmemBytes = kBarOffset + 256 + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory");
 
-// A target that is neither in [0, vocab) nor ignore_index makes its row's lse NaN.
-struct RowInfo {
-    const int64_t* target;
-    int64_t ignore_index;
-    int vocab;
-};
-
 // What a GEMM's epilogue does with its tile.
 enum Kind : int {
     kStats,  // row statistics of the logits
@@ -74,15 +67,22 @@ struct alignas(64) Task {
     int v0;         // kDz: the piece's first column of the vocabulary
 };
 
+// What the epilogues and the row kernels know of the rows.  A target that is neither in [0, V) nor
+// ignore_index makes its row's lse NaN.
 struct Rowwise {
     int64_t T;
     int V;
     const int64_t* target;
-    float2* part;            // kStats: [ceil(V / 128)][T] maximum and sum of each piece of a row
-    float* zt;               // kStats: [T] logit of the target
-    const float* lse;        // kDz
-    const float* row_scale;  // kDz: r_t 2^15 (0 for ignored rows)
-    const float* common;     // kOut: one value
+    int64_t ignore_index;
+    int reduction;
+    float2* part;   // forward: [pieces][T] maximum and sum of each piece of a row
+    float* zt;      // forward: [T] logit of the target
+    uint32_t* done; // forward: the join kernel's count of finished blocks
+    const float* lse;
+    const float* grad;
+    const float* row_scale;  // r_t unit (0 for ignored rows); NULL: unit, or 0
+    float unit;
+    float* common;  // gmax / unit, the factor of the results
 };
 
 constexpr int kMaxTasks = 3;
@@ -169,7 +169,9 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
     const bool live = row < p.T;
     const int64_t y = (live ? p.target[row] : -1) - t.v0;
     const float l2 = live ? p.lse[row] * kLog2e : 0.f;
-    const float rs = live ? p.row_scale[row] : 0.f;
+    const float rs = !live                    ? 0.f
+                     : p.row_scale != nullptr ? p.row_scale[row]
+                                              : (p.target[row] != p.ignore_index ? p.unit : 0.f);
     const int boxes = min(2, (t.N - n0 + 63) / 64);
 #pragma unroll 1
     for (int b = 0; b < boxes; ++b) {
@@ -296,6 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     const int rank = static_cast<int>(cluster_rank());
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int n_items = L.task[L.tasks - 1].items_end;
+    pdl_release();
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kStages);
     const uint32_t acc_full0 = smem_u32(bars + 2 * kStages), acc_empty0 = smem_u32(bars + 2 * kStages + 2);
     const uint32_t drain_bar = smem_u32(bars + 2 * kStages + 4);
@@ -322,6 +325,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    if (L.rows.done != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *L.rows.done = 0u;
 
     if (warp == 0) {
         // ---------------- TMA producer, in both CTAs ----------------
@@ -418,6 +423,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                 umma_commit_pair(acc_full0 + 8);
             }
         }
+        // One idle warp counts the rows of a mean for the launches that scale results by it.
+        if (blockIdx.x == 1 && L.rows.grad != nullptr && L.rows.row_scale == nullptr) {
+            int64_t kept = 0;
+            if (L.rows.reduction == MORPHO_REDUCTION_MEAN) {
+#pragma unroll 8
+                for (int64_t i = lane; i < L.rows.T; i += 32) kept += L.rows.target[i] != L.rows.ignore_index;
+                for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+            }
+            if (lane == 0) *L.rows.common = *L.rows.grad / (static_cast<float>(max(kept, int64_t(1))) * L.rows.unit);
+        }
     } else {
         // ---------------- epilogue, in both CTAs ----------------
         const int quad = warp & 3, half = (warp - 2) >> 2;
@@ -466,6 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
 template <bool BF16>
 __global__ void __launch_bounds__(256) vocab_finish_kernel(const float* part, int slabs, int64_t elems, const float* common,
                                                            uint16_t* out) {
+    pdl_release();
+    pdl_wait();
     const float g = *common;
     for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < elems; i += static_cast<int64_t>(gridDim.x) * 2048) {
         float4 a = *reinterpret_cast<const float4*>(part + i), b = *reinterpret_cast<const float4*>(part + i + 4);
@@ -479,96 +496,232 @@ __global__ void __launch_bounds__(256) vocab_finish_kernel(const float* part, in
     }
 }
 
-// ---- small kernels ------------------------------------------------------------------------------
+// ---- a few tokens: logits on CUDA cores ------------------------------------------------------------
 
-// Joins a row's pieces: lse = m + log(sum_i s_i exp(m_i - m)); loss = lse - z_target.  32 rows per block,
-// eight threads a row.
-__global__ void __launch_bounds__(256) vocab_join_kernel(const float2* part, int pieces, int64_t T, const float* zt,
-                                                         RowInfo info, float* loss, float* lse) {
-    __shared__ float2 sh[8][33];
-    const int rx = threadIdx.x & 31, py = threadIdx.x >> 5;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + rx;
-    float m = -INFINITY, s = 0.f;
-    auto join = [&](float2 o) {
-        const float mn = fmaxf(m, o.x);
-        if (mn > -INFINITY) {
-            s = s * expf(m - mn) + o.y * expf(o.x - mn);
-            m = mn;
-        } else {
-            s += o.y;  // NaN, or nothing
-        }
-    };
-    if (row < T)
-        for (int i = py; i < pieces; i += 8) join(part[i * T + row]);
-    sh[py][rx] = make_float2(m, s);
-    __syncthreads();
-    if (py != 0 || row >= T) return;
-    for (int i = 1; i < 8; ++i) join(sh[i][rx]);
-    const int64_t y = info.target[row];
-    const bool ignored = y == info.ignore_index;
-    float l = m + logf(s);
-    if (!ignored && (y < 0 || y >= info.vocab)) l = NAN;
-    lse[row] = l;
-    loss[row] = ignored ? 0.f : l - zt[row];
-}
+constexpr int kFewTokens = 4;
+constexpr int kFewThreads = 256;
+constexpr int kFewRows = 4;  // vocabulary rows a warp reads at a time
 
-__device__ __forceinline__ double block_total(double x, double* scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-    __syncthreads();
-    double r = 0.0;
-    for (int i = 0; i < static_cast<int>(blockDim.x) / 32; ++i) r += scratch[i];
-    __syncthreads();
-    return r;
-}
-
-// One block: the sum or mean of the rows' losses.
-__global__ void __launch_bounds__(1024) vocab_reduce_kernel(const float* rows, int64_t T, RowInfo info, bool mean,
-                                                            float* out) {
-    __shared__ double scratch[32];
-    double sum = 0.0, kept = 0.0;
-    for (int64_t i = threadIdx.x; i < T; i += 1024) {
-        sum += rows[i];
-        kept += info.target[i] != info.ignore_index ? 1.0 : 0.0;
-    }
-    sum = block_total(sum, scratch);
-    kept = block_total(kept, scratch);
-    if (threadIdx.x == 0) *out = static_cast<float>(mean ? sum / fmax(kept, 1.0) : sum);
-}
-
-// One block: splits the rows' gradients g_t into the factor that dz carries (row_scale = r_t unit) and
-// the common one of the results (*common = gmax / unit).
-__global__ void __launch_bounds__(1024) vocab_scale_kernel(const float* grad, int64_t T, RowInfo info, int reduction,
-                                                           float unit, float* row_scale, float* common) {
-    __shared__ double scratch[32];
-    __shared__ float top[32];
-    float most = 0.f;
-    double kept = 0.0;
-    for (int64_t i = threadIdx.x; i < T; i += 1024) {
-        const bool keep = info.target[i] != info.ignore_index;
-        kept += keep ? 1.0 : 0.0;
-        if (keep && reduction == MORPHO_REDUCTION_NONE) {
-            const float g = fabsf(grad[i]);
-            most = isfinite(g) ? fmaxf(most, g) : most;
-        }
-    }
-    kept = block_total(kept, scratch);
-    if (reduction == MORPHO_REDUCTION_NONE) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = most;
-        __syncthreads();
-        for (int i = 0; i < 32; ++i) most = fmaxf(most, top[i]);
-        if (most == 0.f) most = 1.f;
+// (m, s) <- (m, s) joined with (om, os): m the maximum, s the sum of exp(z - m).
+__device__ __forceinline__ void join(float& m, float& s, float om, float os) {
+    const float mn = fmaxf(m, om);
+    if (mn > -INFINITY) {
+        s = s * ex2((m - mn) * kLog2e) + os * ex2((om - mn) * kLog2e);
+        m = mn;
     } else {
-        most = reduction == MORPHO_REDUCTION_MEAN ? static_cast<float>(*grad / fmax(kept, 1.0)) : *grad;
+        s += os;  // NaN, or nothing
     }
-    for (int64_t i = threadIdx.x; i < T; i += 1024) {
-        const bool keep = info.target[i] != info.ignore_index;
-        row_scale[i] = !keep ? 0.f : reduction == MORPHO_REDUCTION_NONE ? grad[i] / most * unit : unit;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void unpack8(uint4 x, float* f) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (BF16) {
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        } else {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            f[2 * i] = v.x;
+            f[2 * i + 1] = v.y;
+        }
     }
-    if (threadIdx.x == 0) *common = most / unit;
+}
+
+// Up to TT tokens against the whole vocabulary, bound by reading the weight once: each warp takes a
+// contiguous range of its rows, kFewRows at a time, the hidden rows stand in shared memory, and every
+// CTA leaves one piece of each token's statistics.
+template <bool BF16, int TT>
+__global__ void __launch_bounds__(kFewThreads) vocab_few_kernel(const Rowwise p, const uint16_t* hidden, int64_t ldh,
+                                                                const uint16_t* weight, int64_t ldw, int D) {
+    extern __shared__ uint4 hs[];  // [TT][D / 8]
+    __shared__ float2 sh[kFewThreads / 32][TT];
+    pdl_release();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, T = static_cast<int>(p.T), chunks = D / 8;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0u;
+    for (int i = threadIdx.x; i < TT * chunks; i += kFewThreads) {
+        const int t = i / chunks;
+        hs[i] = t < T ? *reinterpret_cast<const uint4*>(hidden + t * ldh + (i - t * chunks) * 8) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    int64_t y[TT];
+    float m[TT], s[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        y[t] = t < T ? p.target[t] : -1;
+        m[t] = -INFINITY;
+        s[t] = 0.f;
+    }
+    const int warps = gridDim.x * (kFewThreads / 32);
+    const int per = (p.V + warps - 1) / warps;
+    const int v0 = min(static_cast<int64_t>(p.V), static_cast<int64_t>(blockIdx.x * (kFewThreads / 32) + warp) * per);
+    const int v1 = min(static_cast<int64_t>(p.V), static_cast<int64_t>(v0) + per);
+    for (int v = v0; v < v1; v += kFewRows) {
+        float acc[kFewRows][TT];
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[r][t] = 0.f;
+        const uint16_t* w = weight + static_cast<int64_t>(v) * ldw;
+#pragma unroll 2
+        for (int c = lane; c < chunks; c += 32) {
+            uint4 x[kFewRows];
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r)
+                x[r] = v + r < v1 ? __ldcs(reinterpret_cast<const uint4*>(w + r * ldw + c * 8)) : make_uint4(0, 0, 0, 0);
+            float h[TT][8];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) unpack8<BF16>(hs[t * chunks + c], h[t]);
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r) {
+                float f[8];
+                unpack8<BF16>(x[r], f);
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) acc[r][t] = fmaf(f[k], h[t][k], acc[r][t]);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) acc[r][t] += __shfl_xor_sync(0xffffffffu, acc[r][t], o);
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                if (v + r < v1) {
+                    join(m[t], s[t], acc[r][t], acc[r][t] == acc[r][t] ? 1.f : acc[r][t]);
+                    if (lane == 0 && y[t] == v + r) p.zt[t] = acc[r][t];
+                }
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+        if (lane == 0) sh[warp][t] = make_float2(m[t], s[t]);
+    __syncthreads();
+    if (threadIdx.x < T) {
+        const int t = threadIdx.x;
+        float mm = -INFINITY, ss = 0.f;
+        for (int i = 0; i < kFewThreads / 32; ++i) join(mm, ss, sh[i][t].x, sh[i][t].y);
+        p.part[static_cast<int64_t>(blockIdx.x) * T + t] = make_float2(mm, ss);
+    }
+}
+
+// ---- row kernels ------------------------------------------------------------------------------------
+
+constexpr int kJoinThreads = 256;
+
+// Joins a row's pieces: lse = m + log(sum_i s_i exp(m_i - m)); loss = lse - z_target.  R rows a block,
+// kJoinThreads / R threads a row, in a fixed order.  For a sum or a mean, each block leaves its rows'
+// sum and the block that ends last adds those up, again in a fixed order.
+template <int R>
+__global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const Rowwise p, int pieces, double2* block_sums, float* loss, float* lse) {
+    constexpr int P = kJoinThreads / R;
+    __shared__ float2 sh[kJoinThreads];
+    __shared__ double2 sums[kJoinThreads / 32];
+    __shared__ bool last;
+    pdl_release();
+    pdl_wait();
+    const int rx = threadIdx.x % R, py = threadIdx.x / R;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * R + rx;
+    float m = -INFINITY, s = 0.f;
+    if (row < p.T) {
+        int i = py;
+        for (; i + 3 * P < pieces; i += 4 * P) {
+            float2 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = p.part[(static_cast<int64_t>(i) + k * P) * p.T + row];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) join(m, s, o[k].x, o[k].y);
+        }
+        for (; i < pieces; i += P) {
+            const float2 o = p.part[static_cast<int64_t>(i) * p.T + row];
+            join(m, s, o.x, o.y);
+        }
+    }
+    sh[threadIdx.x] = make_float2(m, s);
+#pragma unroll
+    for (int n = P / 2; n > 0; n >>= 1) {
+        __syncthreads();
+        if (py < n) {
+            const float2 o = sh[threadIdx.x + n * R];
+            join(m, s, o.x, o.y);
+            sh[threadIdx.x] = make_float2(m, s);
+        }
+    }
+    double l = 0.0, kept = 0.0;
+    if (py == 0 && row < p.T) {
+        const int64_t y = p.target[row];
+        const bool ignored = y == p.ignore_index;
+        float e = m + logf(s);
+        if (!ignored && (y < 0 || y >= p.V)) e = NAN;
+        lse[row] = e;
+        const float one = ignored ? 0.f : e - p.zt[row];
+        if (p.reduction == MORPHO_REDUCTION_NONE) loss[row] = one;
+        l = one;
+        kept = ignored ? 0.0 : 1.0;
+    }
+    if (p.reduction == MORPHO_REDUCTION_NONE) return;
+    auto block_sum = [&]() {  // into thread 0
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
+            kept += __shfl_xor_sync(0xffffffffu, kept, o);
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = make_double2(l, kept);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 1; i < kJoinThreads / 32; ++i) {
+                l += sums[i].x;
+                kept += sums[i].y;
+            }
+    };
+    block_sum();
+    if (threadIdx.x == 0) {
+        block_sums[blockIdx.x] = make_double2(l, kept);
+        __threadfence();
+        last = atomicAdd(p.done, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    l = kept = 0.0;
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += kJoinThreads) {
+        const double2 o = __ldcg(block_sums + i);
+        l += o.x;
+        kept += o.y;
+    }
+    block_sum();
+    if (threadIdx.x == 0) *loss = static_cast<float>(p.reduction == MORPHO_REDUCTION_MEAN ? l / fmax(kept, 1.0) : l);
+}
+
+// Per-token gradients, one block: splits g_t into the factor that dz carries (row_scale = r_t unit) and
+// the common one of the results (*common = gmax / unit).
+__global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, float* row_scale) {
+    __shared__ float top[32];
+    pdl_release();
+    pdl_wait();
+    float most = 0.f;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < p.T; i += 1024) {
+        const float g = fabsf(p.grad[i]);
+        if (p.target[i] != p.ignore_index && isfinite(g)) most = fmaxf(most, g);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = most;
+    __syncthreads();
+    for (int i = 0; i < 32; ++i) most = fmaxf(most, top[i]);
+    if (most == 0.f) most = 1.f;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < p.T; i += 1024)
+        row_scale[i] = p.target[i] != p.ignore_index ? p.grad[i] / most * p.unit : 0.f;
+    if (threadIdx.x == 0) *p.common = most / p.unit;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -644,15 +797,38 @@ struct Bump {
     }
 };
 
+int64_t few_width(int64_t T) { return T <= 2 ? T : 4; }  // tokens that the kernel for T tokens is made for
+
+// Up to kFewTokens tokens skip the tensor cores; their pieces are the CTAs.
+bool few(const morpho_vocab_loss_t* p) {
+    return p->tokens <= kFewTokens && few_width(p->tokens) * p->dim * 2 <= 40 * 1024;  // the hidden rows' shared memory
+}
+
+int few_blocks(const morpho_vocab_loss_t* p, int sms) {
+    return static_cast<int>(std::min<int64_t>(ceil_div(p->vocab, kFewRows * kFewThreads / 32), 3 * sms));
+}
+
+int join_rows(int64_t T, int sms) {  // rows a block of the join takes: a power of two up to 32
+    int r = 1;
+    while (r < 32 && T > static_cast<int64_t>(r) * 2 * sms) r *= 2;
+    return r;
+}
+
 struct FwdPlan {
+    int pieces, rows;
     float2* part;
-    float *zt, *rows;
+    float* zt;
+    double2* sums;
+    uint32_t* done;
 };
-void plan_forward(Bump& b, const morpho_vocab_loss_t* p, FwdPlan* f) {
-    const size_t T = p->tokens, pieces = (p->vocab + kHalf - 1) / kHalf;
-    f->part = b.take<float2>(pieces * T);
+void plan_forward(Bump& b, const morpho_vocab_loss_t* p, int sms, FwdPlan* f) {
+    const size_t T = p->tokens;
+    f->pieces = few(p) ? few_blocks(p, sms) : static_cast<int>(ceil_div(p->vocab, kHalf));
+    f->rows = join_rows(T, sms);
+    f->part = b.take<float2>(f->pieces * T);
     f->zt = b.take<float>(T);
-    f->rows = b.take<float>(T);
+    f->sums = b.take<double2>(ceil_div(T, f->rows));
+    f->done = b.take<uint32_t>(1);
 }
 
 struct BwdPlan {
@@ -721,7 +897,7 @@ int launch(const DeviceInfo& dev, Launch& L, cudaStream_t stream, const char* na
     L.status = dev.status;
     const int pairs = std::min(L.task[L.tasks - 1].items_end, std::max(1, dev.sms / 2));
     prof_begin(stream, name);
-    kern<<<2 * pairs, kGemmThreads, kSmemBytes, stream>>>(L);
+    MORPHO_CUDA_TRY(launch_after(kern, 2 * pairs, kGemmThreads, kSmemBytes, stream, L));
     MORPHO_LAUNCH_CHECK(name);
     return MORPHO_OK;
 }
@@ -730,57 +906,90 @@ template <bool BF16>
 int finish(const DeviceInfo& dev, const float* part, int slabs, int64_t elems, const float* common, void* out, cudaStream_t stream) {
     prof_begin(stream, "vocab_finish");
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(ceil_div(elems, 2048), 8 * dev.sms));
-    vocab_finish_kernel<BF16><<<grid, 256, 0, stream>>>(part, slabs, elems, common, static_cast<uint16_t*>(out));
+    MORPHO_CUDA_TRY(launch_after(vocab_finish_kernel<BF16>, grid, 256, 0, stream, part, slabs, elems, common, static_cast<uint16_t*>(out)));
     MORPHO_LAUNCH_CHECK("vocab_finish");
     return MORPHO_OK;
 }
 
-template <bool BF16>
-int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* hidden, const void* weight,
-              const RowInfo& info, float* loss, float* lse, const FwdPlan& f, cudaStream_t stream) {
-    Launch L{};
-    L.rows.T = p->tokens;
-    L.rows.V = p->vocab;
-    L.rows.target = info.target;
-    L.rows.part = f.part;
-    L.rows.zt = f.zt;
-    Task t{};
-    MORPHO_TRY(load_map(&t.a, hidden, p->tokens, p->dim, ld_hidden(p), false));
-    MORPHO_TRY(load_map(&t.b, weight, p->vocab, p->dim, ld_weight(p), false));
-    MORPHO_TRY(add_task(&L, t, kStats, false, false, p->tokens, p->vocab, p->dim, 1));
-    MORPHO_TRY(launch<BF16>(dev, L, stream, "vocab_stats"));
-    const bool none = p->reduction == MORPHO_REDUCTION_NONE;
-    prof_begin(stream, "vocab_join");
-    vocab_join_kernel<<<static_cast<unsigned>((p->tokens + 31) / 32), 256, 0, stream>>>(
-        f.part, (p->vocab + kHalf - 1) / kHalf, p->tokens, f.zt, info, none ? loss : f.rows, lse);
-    MORPHO_LAUNCH_CHECK("vocab_join");
-    if (!none) {
-        prof_begin(stream, "vocab_reduce");
-        vocab_reduce_kernel<<<1, 1024, 0, stream>>>(f.rows, p->tokens, info, p->reduction == MORPHO_REDUCTION_MEAN, loss);
-        MORPHO_LAUNCH_CHECK("vocab_reduce");
-    }
+template <bool BF16, int TT>
+int launch_few(const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks, cudaStream_t stream) {
+    prof_begin(stream, "vocab_few");
+    MORPHO_CUDA_TRY(launch_after(vocab_few_kernel<BF16, TT>, blocks, kFewThreads, static_cast<size_t>(TT) * p->dim * 2, stream, r,
+                                 static_cast<const uint16_t*>(hidden), ld_hidden(p), static_cast<const uint16_t*>(weight), ld_weight(p), p->dim));
+    MORPHO_LAUNCH_CHECK("vocab_few");
     return MORPHO_OK;
+}
+
+int launch_join(const Rowwise& r, const FwdPlan& f, float* loss, float* lse, cudaStream_t stream) {
+    prof_begin(stream, "vocab_join");
+    const unsigned grid = static_cast<unsigned>(ceil_div(r.T, f.rows));
+    auto go = [&](auto kern) { return launch_after(kern, grid, kJoinThreads, 0, stream, r, f.pieces, f.sums, loss, lse); };
+    MORPHO_CUDA_TRY(f.rows == 1    ? go(vocab_join_kernel<1>)
+                    : f.rows == 2  ? go(vocab_join_kernel<2>)
+                    : f.rows == 4  ? go(vocab_join_kernel<4>)
+                    : f.rows == 8  ? go(vocab_join_kernel<8>)
+                    : f.rows == 16 ? go(vocab_join_kernel<16>)
+                                   : go(vocab_join_kernel<32>));
+    MORPHO_LAUNCH_CHECK("vocab_join");
+    return MORPHO_OK;
+}
+
+Rowwise rows_of(const morpho_vocab_loss_t* p, const int64_t* target) {
+    Rowwise r{};
+    r.T = p->tokens;
+    r.V = p->vocab;
+    r.target = target;
+    r.ignore_index = p->ignore_index;
+    r.reduction = p->reduction;
+    return r;
+}
+
+template <bool BF16>
+int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, const int64_t* target,
+              float* loss, float* lse, const FwdPlan& f, cudaStream_t stream) {
+    Rowwise r = rows_of(p, target);
+    r.part = f.part;
+    r.zt = f.zt;
+    r.done = f.done;
+    if (few(p)) {
+        MORPHO_TRY(p->tokens == 1   ? (launch_few<BF16, 1>(r, p, hidden, weight, f.pieces, stream))
+                   : p->tokens == 2 ? (launch_few<BF16, 2>(r, p, hidden, weight, f.pieces, stream))
+                                    : (launch_few<BF16, 4>(r, p, hidden, weight, f.pieces, stream)));
+    } else {
+        Launch L{};
+        L.rows = r;
+        Task t{};
+        MORPHO_TRY(load_map(&t.a, hidden, p->tokens, p->dim, ld_hidden(p), false));
+        MORPHO_TRY(load_map(&t.b, weight, p->vocab, p->dim, ld_weight(p), false));
+        MORPHO_TRY(add_task(&L, t, kStats, false, false, p->tokens, p->vocab, p->dim, 1));
+        MORPHO_TRY(launch<BF16>(dev, L, stream, "vocab_stats"));
+    }
+    return launch_join(r, f, loss, lse, stream);
 }
 
 // One launch computes dz of piece i + 1 beside the two products that read dz of piece i (the two dz
 // buffers alternate), so the tiles of all three fill the SMs together.
 template <bool BF16>
 int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float* grad, const void* hidden, const void* weight,
-               const RowInfo& info, const float* lse, void* dhidden, void* dweight, const BwdPlan& f, cudaStream_t stream) {
-    prof_begin(stream, "vocab_scale");
-    vocab_scale_kernel<<<1, 1024, 0, stream>>>(grad, p->tokens, info, p->reduction, BF16 ? 1.0f : 32768.0f, f.row_scale, f.common);
-    MORPHO_LAUNCH_CHECK("vocab_scale");
+               const int64_t* target, const float* lse, void* dhidden, void* dweight, const BwdPlan& f, cudaStream_t stream) {
+    Rowwise r = rows_of(p, target);
+    r.lse = lse;
+    r.grad = grad;
+    r.unit = BF16 ? 1.0f : 32768.0f;
+    r.common = f.common;
+    if (p->reduction == MORPHO_REDUCTION_NONE) {
+        prof_begin(stream, "vocab_scale");
+        MORPHO_CUDA_TRY(launch_after(vocab_scale_kernel, 1, 1024, 0, stream, r, f.row_scale));
+        MORPHO_LAUNCH_CHECK("vocab_scale");
+        r.row_scale = f.row_scale;
+    }
     const Cut& c = f.cut;
     const int64_t T = p->tokens, D = p->dim;
     auto width = [&](int i) { return std::min<int64_t>(c.cols, p->vocab - static_cast<int64_t>(i) * c.cols); };
     for (int i = -1; i < c.pieces; ++i) {
         Launch L{};
-        L.rows.T = T;
-        L.rows.V = p->vocab;
-        L.rows.target = info.target;
-        L.rows.lse = lse;
-        L.rows.row_scale = f.row_scale;
-        L.rows.common = f.common;
+        L.rows = r;
+        if (i >= 0) L.rows.grad = nullptr;  // the first launch makes *common
         if (i >= 0) {
             const int v0 = i * c.cols;
             const int64_t n = width(i);
@@ -839,7 +1048,7 @@ extern "C" MORPHO_API size_t morpho_sm100_linear_cross_entropy_forward_workspace
     if (validate_loss(p) != MORPHO_OK) return 0;
     Bump b{nullptr};
     FwdPlan f;
-    plan_forward(b, p, &f);
+    plan_forward(b, p, sm_count(), &f);
     return b.off + 256;
 }
 
@@ -875,10 +1084,9 @@ extern "C" MORPHO_API int morpho_sm100_linear_cross_entropy_forward(const morpho
     MORPHO_TRY(current_device_info(&dev));
     Bump b{static_cast<uint8_t*>(workspace)};
     FwdPlan f;
-    plan_forward(b, p, &f);
-    const RowInfo info{target, p->ignore_index, p->vocab};
-    return p->type == MORPHO_DTYPE_BF16 ? forward_t<true>(dev, p, hidden, weight, info, loss, lse, f, st)
-                                        : forward_t<false>(dev, p, hidden, weight, info, loss, lse, f, st);
+    plan_forward(b, p, dev.sms, &f);
+    return p->type == MORPHO_DTYPE_BF16 ? forward_t<true>(dev, p, hidden, weight, target, loss, lse, f, st)
+                                        : forward_t<false>(dev, p, hidden, weight, target, loss, lse, f, st);
 }
 
 extern "C" MORPHO_API int morpho_sm100_linear_cross_entropy_backward(const morpho_vocab_loss_t* p, const float* grad_loss,
@@ -908,7 +1116,6 @@ extern "C" MORPHO_API int morpho_sm100_linear_cross_entropy_backward(const morph
     Bump b{static_cast<uint8_t*>(workspace)};
     BwdPlan f;
     plan_backward(b, p, dev.sms, &f);
-    const RowInfo info{target, p->ignore_index, p->vocab};
-    return p->type == MORPHO_DTYPE_BF16 ? backward_t<true>(dev, p, grad_loss, hidden, weight, info, lse, dhidden, dweight, f, st)
-                                        : backward_t<false>(dev, p, grad_loss, hidden, weight, info, lse, dhidden, dweight, f, st);
+    return p->type == MORPHO_DTYPE_BF16 ? backward_t<true>(dev, p, grad_loss, hidden, weight, target, lse, dhidden, dweight, f, st)
+                                        : backward_t<false>(dev, p, grad_loss, hidden, weight, target, lse, dhidden, dweight, f, st);
 }
