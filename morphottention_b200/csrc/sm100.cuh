@@ -68,6 +68,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // As mbar_try_wait, but lets the hardware park the thread for up to hint_ns while the
 // phase is incomplete (it resumes as soon as the phase completes), so a waiting warp does
 // not spin and take issue slots from the warps doing the work.
@@ -405,12 +418,18 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-// mbar_wait for a barrier that threads of the other CTA arrive at.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t* status, uint32_t kernel,
-                                                  uint32_t site) {
-    const bool ok = mbar_wait(bar, parity, status, kernel, site);
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    return ok;
+// Writes 16 bytes to shared memory of either CTA of the cluster and completes as many on a barrier
+// there, whose waiters then see them (addresses as cluster_addr gives them); and the arrival at that
+// barrier that announces the bytes.
+__device__ __forceinline__ void st_async_v4(uint32_t cluster_dst, uint32_t cluster_bar, int a, int b, int c, int d) {
+    asm volatile(
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.s32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(cluster_dst),
+        "r"(cluster_bar), "r"(a), "r"(b), "r"(c), "r"(d)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes)
+                 : "memory");
 }
 
 // A TMA load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
@@ -420,6 +439,15 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
         "{%3, %4}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0,
+                                                 int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 

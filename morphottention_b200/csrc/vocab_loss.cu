@@ -18,8 +18,8 @@
 //
 // The GEMMs run as 256 x 256 tiles of CTA pairs (cta_group::2): each SM reads half of A's rows and half of
 // B's columns, 32 KB for every 64 of K, where a 128 x 256 tile of one CTA reads 48 KB and leaves its
-// shared memory port busier than its tensor core.  Warp roles (320 threads): warp 0 TMA producer, warp 1
-// MMA issuer (rank 0 of the pair), warps 2-9 epilogue; the accumulator is double-buffered in TMEM, and
+// shared memory port busier than its tensor core.  Warp roles (352 threads): warp 0 TMA producer, warp 1
+// MMA issuer (rank 0 of the pair), warps 2-9 epilogue, warp 10 scheduler; the accumulator is double-buffered in TMEM, and
 // results leave through TMA stores from a swizzled box per warp.
 #include <algorithm>
 
@@ -33,16 +33,15 @@ namespace {
 constexpr uint32_t K_VOCAB = 6;  // kernel id in the device status word
 constexpr int kTile = 256;       // rows and columns of a CTA pair's tile
 constexpr int kHalf = 128;       // rows of A, columns of B, and rows of the tile that one CTA holds
-constexpr int BK = 64;
-constexpr int kGemmThreads = 320;
+constexpr int BK = 128;          // K of a stage
+constexpr int kGemmThreads = 352;
 constexpr int kStages = 3;
-constexpr int kUnits = 2;  // K blocks of 64 in a stage
-constexpr int kOperandBytes = kHalf * BK * 2;
-constexpr int kUnitBytes = 2 * kOperandBytes;
-constexpr int kStageBytes = kUnits * kUnitBytes;
+constexpr int kPanel = kHalf * 128;         // 16 KB: 128 rows of 128 bytes
+constexpr int kOperandBytes = 2 * kPanel;   // 128 x 128 elements: two panels side by side
+constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kStoreOffset = kStages * kStageBytes;  // a 4 KB box for each epilogue warp's stores
 constexpr int kBarOffset = kStoreOffset + 8 * 4096;
-constexpr int kSmemBytes = kBarOffset + 256 + 1024;
+constexpr int kSmemBytes = kBarOffset + 512 + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory");
 
 // What a GEMM's epilogue does with its tile.
@@ -59,10 +58,11 @@ struct alignas(64) Task {
     CUtensorMap a, b, out;
     int kind;
     bool a_mn, b_mn;     // stored [K, M] / [K, N] (else [M, K] / [N, K])
+    bool a_whole, b_whole;  // the map loads both panels of a stage at once (see load_map)
     int a_row0, b_row0;  // first row of A / B in its map
     int M, N;
     int tiles_m, tiles_n, group;  // `group` M tiles share each B tile in L2
-    int k_blocks, kb_per_split;
+    int K, k_blocks, kb_per_split;
     int items_end;  // work items of this task and those before it
     int v0;         // kDz: the piece's first column of the vocabulary
 };
@@ -90,6 +90,9 @@ struct Launch {
     Task task[kMaxTasks];
     int tasks;
     Rowwise rows;
+    uint32_t* next;  // work items taken after the first of each pair; NULL: dealt round-robin
+    uint32_t* zero;  // counters of later launches to clear
+    int zeros;
     uint32_t* status;
 };
 
@@ -116,49 +119,54 @@ __device__ __forceinline__ void stage_box(uint32_t stage, int lane, const uint32
     __syncwarp();
 }
 
-// Row statistics: the piece's maximum and sum of exp(z - maximum), and the target's logit.
+// The warp's 128 columns of its 32 rows, after which the accumulator may be written again.
+template <class Release>
+__device__ __forceinline__ void load_piece(uint32_t tacc, uint32_t* r, Release release) {
+#pragma unroll
+    for (int c = 0; c < kHalf; c += 32) tmem_ld32(tacc + c, r + c);
+    tmem_ld_wait();
+    release();
+}
+
+// Row statistics: the piece's maximum and sum of exp(z - maximum), and the target's logit.  Four
+// independent chains each for the maximum and the sum: two warps per scheduler hide little latency.
 template <class Release>
 __device__ __forceinline__ void epi_stats(const Rowwise& p, uint32_t tacc, int64_t row, int n0, Release release) {
-    const int64_t y = row < p.T ? p.target[row] : -1;
-    float m = -INFINITY, s = 0.f, zt = 0.f;
-#pragma unroll 1
-    for (int cc = 0; cc < kHalf; cc += 32) {
-        uint32_t r[32];
-        __syncwarp();
-        tmem_ld32(tacc + cc, r);
-        tmem_ld_wait();
-        if (cc + 32 == kHalf) release();
-        const int left = p.V - n0 - cc;  // live columns from here on
-        float mx = -INFINITY;
+    const int64_t y = (row < p.T ? p.target[row] : -1) - n0;
+    uint32_t r[kHalf];
+    load_piece(tacc, r, release);
+    if (n0 + kHalf > p.V) {  // columns past the vocabulary
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if (i >= left) r[i] = __float_as_uint(-INFINITY);
-            mx = fmaxf(mx, u2f(r[i]));
-        }
-        const float mn = fmaxf(m, mx);
-        if (mn > -INFINITY) {
-            const float b = mn * kLog2e;
-            float t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) t += ex2(fmaf(u2f(r[i]), kLog2e, -b));
-            s = s * ex2(fmaf(m, kLog2e, -b)) + t;
-            m = mn;
-        } else {
-            // -inf throughout, or NaN (which a maximum skips)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (u2f(r[i]) != u2f(r[i])) s = u2f(r[i]);
-        }
-        const int64_t at = y - n0 - cc;
-        if (at >= 0 && at < 32) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if (i == at) zt = u2f(r[i]);
-        }
+        for (int i = 0; i < kHalf; ++i)
+            if (i >= p.V - n0) r[i] = __float_as_uint(-INFINITY);
     }
+    float m4[4], s4[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        m4[c] = u2f(r[c]);
+        s4[c] = 0.f;
+    }
+#pragma unroll
+    for (int i = 4; i + 8 <= kHalf; i += 8)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m4[c] = fmax3(m4[c], u2f(r[i + c]), u2f(r[i + 4 + c]));
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], u2f(r[kHalf - 4 + c]));
+    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    float zt = 0.f;
+    if (__any_sync(0xffffffffu, y >= 0 && y < kHalf)) {
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+            if (i == y) zt = u2f(r[i]);
+    }
+    const float b = m > -INFINITY ? m * kLog2e : 0.f;  // -inf throughout, or NaN (which a maximum skips)
+#pragma unroll
+    for (int i = 0; i < kHalf; i += 4)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s4[c] += ex2(fmaf(u2f(r[i + c]), kLog2e, -b));
     if (row < p.T) {
-        p.part[static_cast<int64_t>(n0 / kHalf) * p.T + row] = make_float2(m, s);
-        if (y >= n0 && y < n0 + kHalf && y < p.V) p.zt[row] = zt;
+        p.part[static_cast<int64_t>(n0 / kHalf) * p.T + row] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
+        if (y >= 0 && y < kHalf && y + n0 < p.V) p.zt[row] = zt;
     }
 }
 
@@ -167,41 +175,41 @@ template <bool BF16, class Release>
 __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t tacc, int64_t row, int row0, int n0,
                                        uint32_t stage, int lane, Release release) {
     const bool live = row < p.T;
-    const int64_t y = (live ? p.target[row] : -1) - t.v0;
+    const int64_t target = live ? p.target[row] : -1;
+    const int64_t y = target - t.v0 - n0;
     const float l2 = live ? p.lse[row] * kLog2e : 0.f;
     const float rs = !live                    ? 0.f
                      : p.row_scale != nullptr ? p.row_scale[row]
-                                              : (p.target[row] != p.ignore_index ? p.unit : 0.f);
-    const int boxes = min(2, (t.N - n0 + 63) / 64);
-#pragma unroll 1
-    for (int b = 0; b < boxes; ++b) {
-        uint32_t x[32];
+                                              : (target != p.ignore_index ? p.unit : 0.f);
+    uint32_t r[kHalf];
+    load_piece(tacc, r, release);
+    const bool hit = __any_sync(0xffffffffu, y >= 0 && y < kHalf);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            uint32_t r[32];
-            __syncwarp();
-            tmem_ld32(tacc + b * 64 + q * 32, r);
-            tmem_ld_wait();
-            if (q == 1 && b == boxes - 1) release();
-            float d[32];
+    for (int b = 0; b < 2; ++b) {
+        if (n0 + b * 64 < t.N) {
+            uint32_t x[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) d[i] = rs * ex2(fmaf(u2f(r[i]), kLog2e, -l2));
-            const int64_t at = y - (n0 + b * 64 + q * 32);
-            if (at >= 0 && at < 32) {
+            for (int i = 0; i < 64; ++i) r[b * 64 + i] = __float_as_uint(rs * ex2(fmaf(u2f(r[b * 64 + i]), kLog2e, -l2)));
+            if (n0 + b * 64 + 64 > t.N) {  // the last panel's columns past the piece are read as K: zeros
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i == at) d[i] -= rs;
+                for (int i = 0; i < 64; ++i)
+                    if (n0 + b * 64 + i >= t.N) r[b * 64 + i] = 0u;
+            }
+            if (hit) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (b * 64 + i == y) r[b * 64 + i] = __float_as_uint(u2f(r[b * 64 + i]) - rs);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                x[q * 16 + i] = pack2<BF16>(d[2 * i], d[2 * i + 1]);
-                if (rs == 0.f) x[q * 16 + i] = 0u;  // an ignored row adds nothing, whatever its logits are
+            for (int i = 0; i < 32; ++i) {
+                x[i] = pack2<BF16>(u2f(r[b * 64 + 2 * i]), u2f(r[b * 64 + 2 * i + 1]));
+                if (rs == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
             }
-        }
-        stage_box(stage, lane, x);
-        if (lane == 0 && row0 < t.M) {
-            tma_store_2d(&t.out, stage, n0 + b * 64, row0);
-            bulk_commit_group();
+            stage_box(stage, lane, x);
+            if (lane == 0 && row0 < t.M) {
+                tma_store_2d(&t.out, stage, n0 + b * 64, row0);
+                bulk_commit_group();
+            }
         }
     }
 }
@@ -258,13 +266,14 @@ __device__ __forceinline__ void epi_part(const Task& t, uint32_t tacc, int row0,
 // ---- the GEMM: up to three tasks in one persistent launch of CTA pairs -----------------------------
 
 struct Item {
-    int task, m0, n0, z, kb0, kb1;
+    int task, m0, n0, z;  // task -1: no more work
 };
 
 // Work item w: the tasks one after the other; within a task the splits, then groups of `group` M tiles,
 // then the N tiles, then the M tiles of the group.
 __device__ __forceinline__ Item item_of(const Launch& L, int w) {
-    Item it;
+    Item it{-1, 0, 0, 0};
+    if (w >= L.task[L.tasks - 1].items_end) return it;
     int i = 0, start = 0;
     while (w >= L.task[i].items_end) start = L.task[i++].items_end;
     const Task& t = L.task[i];
@@ -279,9 +288,73 @@ __device__ __forceinline__ Item item_of(const Launch& L, int w) {
     const int n = r / gm;
     it.m0 = (g * t.group + r - n * gm) * kTile;
     it.n0 = n * kTile;
-    it.kb0 = it.z * t.kb_per_split;
-    it.kb1 = min(t.k_blocks, it.kb0 + t.kb_per_split);
     return it;
+}
+
+__device__ __forceinline__ int first_block(const Task& t, const Item& it) { return it.z * t.kb_per_split; }
+__device__ __forceinline__ int end_block(const Task& t, const Item& it) {
+    return min(t.k_blocks, (it.z + 1) * t.kb_per_split);
+}
+
+// The items a CTA pair works on, published by rank 0's scheduler warp through a ring of kSlots in each CTA
+// and read by the other roles in order.  The first item of a pair is its index, which all roles know.
+// With two slots the scheduler takes an item when the epilogue has begun the last but one: early enough
+// for the loads, late enough that pairs take the last items as they become free.
+constexpr int kSlots = 2;
+struct Items {
+    uint32_t slot0, full0, empty0;  // shared-memory addresses: slots, full barriers; empty barriers (rank 0's)
+
+    // The scheduler: item number n > 0.
+    __device__ void publish(int n, const Item& it) const {
+        const int s = n % kSlots;
+        for (uint32_t r = 0; r < 2; ++r) {
+            const uint32_t bar = cluster_addr(full0 + 8 * s, r);
+            mbar_arrive_expect_tx_cluster(bar, 16);
+            st_async_v4(cluster_addr(slot0 + 16 * s, r), bar, it.task, it.m0, it.n0, it.z);
+        }
+    }
+    // Whether (in time) the slot for item n has been read by all.
+    __device__ bool room(int n, uint32_t* status) const {
+        return n <= kSlots || mbar_wait(empty0 + 8 * (n % kSlots), ((n - 1) / kSlots & 1) ^ 1, status, K_VOCAB, 8);
+    }
+    // Any other role: item number n > 0; false on a timeout.  One thread then calls taken(n).  Where the
+    // items are dealt round-robin every role works them out for itself.
+    __device__ bool read(int n, Item& it, const Launch& L, int first, int step) const {
+        if (L.next == nullptr) {
+            it = item_of(L, first + n * step);
+            return true;
+        }
+        uint32_t* status = L.status;
+        const int s = n % kSlots;
+        if (!mbar_wait(full0 + 8 * s, ((n - 1) / kSlots) & 1, status, K_VOCAB, 9)) return false;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(it.task), "=r"(it.m0), "=r"(it.n0), "=r"(it.z)
+                     : "r"(slot0 + 16 * s)
+                     : "memory");
+        return true;
+    }
+    __device__ void taken(int n, const Launch& L) const {
+        if (L.next != nullptr) mbar_arrive_cluster(cluster_addr(empty0 + 8 * (n % kSlots), 0));
+    }
+};
+
+// One operand of a stage: rows (M or N) x .. x + 127, K k .. k + 127, in two panels of 128 rows of 128 bytes.
+// K-major: the panels are the halves of K; MN-major: the halves of the rows, each with K down.
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap& map, uint32_t bar, bool mn, bool whole, int row0,
+                                             int x, int k) {
+    if (mn) {
+        if (whole) {
+            tma_load_3d_pair(dst, &map, bar, 0, row0 + k, x / 64);
+        } else {
+            tma_load_2d_pair(dst, &map, bar, x, row0 + k);
+            tma_load_2d_pair(dst + kPanel, &map, bar, x + 64, row0 + k);
+        }
+    } else if (whole) {
+        tma_load_3d_pair(dst, &map, bar, 0, row0 + x, k / 64);
+    } else {
+        tma_load_2d_pair(dst, &map, bar, k, row0 + x);
+        tma_load_2d_pair(dst + kPanel, &map, bar, k + 64, row0 + x);
+    }
 }
 
 template <bool BF16>
@@ -289,20 +362,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOffset);
-    constexpr int NB = 2 * kStages + 5;  // full, empty, acc_full[2], acc_empty[2], drain
-    static_assert(NB * 8 + 8 <= 256, "barrier block");
+    // full, empty, acc_full[2], acc_empty[2], drain, item full, item empty
+    constexpr int NB = 2 * kStages + 5 + 2 * kSlots;
+    constexpr int kSlotWord = (NB * 8 + 8 + 15) / 16 * 4;  // first word of the item ring, after the two below
+    static_assert(kSlotWord * 4 + 16 * kSlots <= 512, "barrier block");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     const int warp = warp_id();
     const int lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    const int n_items = L.task[L.tasks - 1].items_end;
     pdl_release();
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kStages);
     const uint32_t acc_full0 = smem_u32(bars + 2 * kStages), acc_empty0 = smem_u32(bars + 2 * kStages + 2);
     const uint32_t drain_bar = smem_u32(bars + 2 * kStages + 4);
+    const Items items{smem_u32(reinterpret_cast<uint32_t*>(bars) + kSlotWord), smem_u32(bars + 2 * kStages + 5), smem_u32(bars + 2 * kStages + 5 + kSlots)};
     if (threadIdx.x == 0) {
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(items.full0 + 8 * s, 1);    // rank 0's scheduler, to both
+            mbar_init(items.empty0 + 8 * s, 19);  // used in rank 0: its MMA thread, 2 producers, 16 epilogue warps
+        }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, 1);   // used in rank 0: its producer's arrival and both CTAs' bytes
             mbar_init(empty0 + 8 * s, 1);  // rank 0's commit, to both
@@ -327,40 +406,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     const uint32_t tmem = *tmem_slot;
     pdl_wait();
     if (L.rows.done != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *L.rows.done = 0u;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < L.zeros; i += kGemmThreads) L.zero[i] = 0u;
 
     if (warp == 0) {
         // ---------------- TMA producer, in both CTAs ----------------
         if (lane == 0) {
             int g = 0;
-            for (int w = first; w < n_items && !*abort_flag; w += step) {
-                const Item it = item_of(L, w);
+            Item it = item_of(L, first);
+            for (int j = 0; !*abort_flag; ++j) {
+                if (j > 0) {
+                    if (!items.read(j, it, L, first, step)) {
+                        *abort_flag = 1u;
+                        break;
+                    }
+                    items.taken(j, L);
+                }
+                if (it.task < 0) break;
                 const Task& t = L.task[it.task];
+                const int kb0 = first_block(t, it), kb1 = end_block(t, it);
                 const int m = it.m0 + rank * kHalf, n = it.n0 + rank * kHalf;
-                for (int kb = it.kb0; kb < it.kb1; kb += kUnits, ++g) {
+                for (int kb = kb0; kb < kb1; ++kb, ++g) {
                     const int s = g % kStages;
                     if (g >= kStages && !mbar_wait(empty0 + 8 * s, ((g / kStages) & 1) ^ 1, L.status, K_VOCAB, 1)) {
                         *abort_flag = 1u;
                         break;
                     }
+                    const uint32_t sA = smem_u32(smem + s * kStageBytes);
                     const uint32_t fb = cluster_addr(full0 + 8 * s, 0);
-                    const int units = min(kUnits, it.kb1 - kb);
-                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, units * 2 * kUnitBytes);
-                    for (int u = 0; u < units; ++u) {
-                        const uint32_t sA = smem_u32(smem + s * kStageBytes + u * kUnitBytes), sB = sA + kOperandBytes;
-                        const int k0 = (kb + u) * BK;
-                        if (t.a_mn) {
-                            tma_load_2d_pair(sA, &t.a, fb, m, t.a_row0 + k0);
-                            tma_load_2d_pair(sA + 64 * 128, &t.a, fb, m + 64, t.a_row0 + k0);
-                        } else {
-                            tma_load_2d_pair(sA, &t.a, fb, k0, t.a_row0 + m);
-                        }
-                        if (t.b_mn) {
-                            tma_load_2d_pair(sB, &t.b, fb, n, t.b_row0 + k0);
-                            tma_load_2d_pair(sB + 64 * 128, &t.b, fb, n + 64, t.b_row0 + k0);
-                        } else {
-                            tma_load_2d_pair(sB, &t.b, fb, k0, t.b_row0 + n);
-                        }
-                    }
+                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * kStageBytes);
+                    load_operand(sA, t.a, fb, t.a_mn, t.a_whole, t.a_row0, m, kb * BK);
+                    load_operand(sA + kOperandBytes, t.b, fb, t.b_mn, t.b_whole, t.b_row0, n, kb * BK);
                 }
             }
             // No CTA leaves while commits to its barriers are on their way.
@@ -377,43 +453,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
         if (rank == 0 && lane == 0) {
             constexpr uint32_t type_bits = BF16 ? (1u << 7) | (1u << 10) : 0u;
             bool ok = true;
-            int g = 0, j = 0;
-            for (int w = first; ok && w < n_items; w += step, ++j) {
-                const Item it = item_of(L, w);
-                const bool a_mn = L.task[it.task].a_mn, b_mn = L.task[it.task].b_mn;
+            int g = 0;
+            Item it = item_of(L, first);
+            for (int j = 0; ok && it.task >= 0; ++j) {
+                const Task& t = L.task[it.task];
+                const bool a_mn = t.a_mn, b_mn = t.b_mn;
+                const int kb0 = first_block(t, it), kb1 = end_block(t, it);
                 const uint32_t idesc = make_idesc_f16(kTile, kTile, a_mn, b_mn) | type_bits;
-                // K-major: 8-row groups of 1 KB, K = 16 every 32 bytes; MN-major: 64-column groups of
-                // 8 KB, 8-row groups of 1 KB, K = 16 every 2 KB
-                const uint32_t a_lbo = a_mn ? 64 * 128 : 16, b_lbo = b_mn ? 64 * 128 : 16;
-                const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
                 const int a = j & 1;
-                if (j >= 2 && !mbar_wait_cluster(acc_empty0 + 8 * a, ((j >> 1) & 1) ^ 1, L.status, K_VOCAB, 6)) {
+                if (j >= 2 && !mbar_wait(acc_empty0 + 8 * a, ((j >> 1) & 1) ^ 1, L.status, K_VOCAB, 6)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t dacc = tmem + a * kTile;
-                for (int i = it.kb0; i < it.kb1; i += kUnits, ++g) {
+                for (int kb = kb0; kb < kb1; ++kb, ++g) {
                     const int s = g % kStages;
                     // (what the TMA wrote needs no tcgen05 fence: the MMAs read it through the async proxy)
                     if (!mbar_wait(full0 + 8 * s, (g / kStages) & 1, L.status, K_VOCAB, 3)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t sA = smem_u32(smem + s * kStageBytes);
+                    const uint32_t sA = smem_u32(smem + s * kStageBytes), sB = sA + kOperandBytes;
+                    const int left = t.K - kb * BK;  // the last stage may hold less: whole K = 16 steps of zeros are left out
 #pragma unroll
-                    for (int u = 0; u < kUnits; ++u) {
-                        if (u == 0 || i + u < it.kb1) {
-#pragma unroll
-                            for (int ks = 0; ks < BK / 16; ++ks)
-                                umma_ss_pair(dacc, make_sdesc(sA + u * kUnitBytes + ks * a_step, a_lbo, 1024, SW_128),
-                                               make_sdesc(sA + u * kUnitBytes + kOperandBytes + ks * b_step, b_lbo, 1024, SW_128), idesc,
-                                               (i > it.kb0 || u > 0 || ks > 0) ? 1u : 0u);
-                        }
+                    for (int ks = 0; ks < BK / 16; ++ks) {
+                        // K-major: K = 16 every 32 bytes of a panel's rows, 8-row groups of 1 KB; MN-major:
+                        // K = 16 every 2 KB, the second 64 rows a panel further
+                        const uint32_t kmaj = (ks / 4) * kPanel + (ks % 4) * 32, mnmaj = ks * 2048;
+                        if (ks * 16 < left)
+                            umma_ss_pair(dacc, make_sdesc(sA + (a_mn ? mnmaj : kmaj), a_mn ? kPanel : 16, 1024, SW_128),
+                                         make_sdesc(sB + (b_mn ? mnmaj : kmaj), b_mn ? kPanel : 16, 1024, SW_128), idesc,
+                                         (kb > kb0 || ks > 0) ? 1u : 0u);
                     }
                     umma_commit_pair(empty0 + 8 * s);
                 }
                 if (ok) umma_commit_pair(acc_full0 + 8 * a);
+                if (ok && !items.read(j + 1, it, L, first, step)) ok = false;
+                if (ok) items.taken(j + 1, L);
             }
             if (!ok) {
                 *abort_flag = 1u;
@@ -433,13 +510,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
             }
             if (lane == 0) *L.rows.common = *L.rows.grad / (static_cast<float>(max(kept, int64_t(1))) * L.rows.unit);
         }
+    } else if (warp == 10) {
+        // ---------------- scheduler, one thread of rank 0 ----------------
+        if (rank == 0 && lane == 0 && L.next != nullptr) {
+            Item it = item_of(L, first);
+            for (int j = 1; it.task >= 0; ++j) {
+                if (!items.room(j, L.status)) {
+                    *abort_flag = 1u;
+                    break;
+                }
+                it = item_of(L, step + static_cast<int>(atomicAdd(L.next, 1u)));
+                items.publish(j, it);
+            }
+        }
     } else {
         // ---------------- epilogue, in both CTAs ----------------
         const int quad = warp & 3, half = (warp - 2) >> 2;
         const uint32_t stage = smem_u32(smem + kStoreOffset + (warp - 2) * 4096);
-        int j = 0;
-        for (int w = first; w < n_items; w += step, ++j) {
-            const Item it = item_of(L, w);
+        Item it = item_of(L, first);
+        for (int j = 0;; ++j) {
+            if (j > 0) {
+                const bool ok = items.read(j, it, L, first, step);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    *abort_flag = 1u;
+                    break;
+                }
+                if (lane == 0) items.taken(j, L);
+            }
+            if (it.task < 0) break;
             const Task& t = L.task[it.task];
             const int a = j & 1;
             if (!mbar_wait_warp(acc_full0 + 8 * a, (j >> 1) & 1, L.status, K_VOCAB, 5) || *abort_flag) {
@@ -726,7 +824,7 @@ __global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, floa
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr size_t kPieceBytes = 256u << 20;  // dz of one piece of the vocabulary, at most; two are held
+constexpr size_t kPieceBytes = 512u << 20;  // dz of one piece of the vocabulary, at most; two are held
 // Terms of one tensor-core sum, at most.  The tensor core truncates its fp32 accumulator at every
 // K = 16 step, which biases a long sum towards zero (2.3e-8 of it a step; 1.2 % measured after 2^23
 // terms), so longer sums are joined from sums of this length by rounded fp32 additions.
@@ -761,10 +859,10 @@ struct Cut {
 
 // K splits of a GEMM of `tiles` tiles and `kb` K blocks in a launch with `total` tile * K-block units on
 // `pairs` CTA pairs: no split longer than kMaxK, nor than a third of a pair's share of the launch (so that
-// uneven shares cost little), nor, for the latter, shorter than 32 blocks (a partial tile costs about as
-// much to write and join as 16 blocks to compute).
+// uneven shares cost little), nor, for the latter, shorter than 16 blocks (a partial tile costs about as
+// much to write and join as 8 blocks to compute).
 int splits_of(int64_t kb, int64_t total, int pairs) {
-    const int64_t share = std::max<int64_t>(32, total / (3 * pairs));
+    const int64_t share = std::max<int64_t>(16, total / (3 * pairs));
     const int64_t splits = ceil_div(kb, std::min<int64_t>(share, kMaxK / BK));
     const int64_t per = ceil_div(kb, splits);
     return static_cast<int>(ceil_div(kb, per));  // no empty split
@@ -778,7 +876,7 @@ Cut cut_of(const morpho_vocab_loss_t* p, int sms) {
     c.cols = static_cast<int>(std::min(all, std::max<int64_t>(kTile, fit)));
     c.pieces = static_cast<int>(ceil_div(p->vocab, c.cols));
     const int64_t tt = ceil_div(T, kTile), tv = c.cols / kTile, td = ceil_div(p->dim, kTile);
-    const int64_t total = tt * tv * ceil_div(p->dim, BK) + tt * td * (c.cols / BK) + tv * td * ceil_div(T, BK);
+    const int64_t total = tt * tv * ceil_div(p->dim, BK) + tt * td * ceil_div(c.cols, BK) + tv * td * ceil_div(T, BK);
     const int pairs = std::max(1, sms / 2);
     c.splits_h = splits_of(ceil_div(std::min<int64_t>(c.cols, p->vocab), BK), total, pairs);
     c.splits_w = splits_of(ceil_div(T, BK), total, pairs);
@@ -835,6 +933,7 @@ struct BwdPlan {
     Cut cut;
     uint16_t* dz[2];
     float *row_scale, *common, *hpart, *wpart;
+    uint32_t* next;  // a work counter for each launch after the first
 };
 void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
     f->cut = cut_of(p, sms);
@@ -842,7 +941,8 @@ void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
     const size_t T = p->tokens, D = p->dim;
     for (int i = 0; i < 2; ++i) f->dz[i] = b.take<uint16_t>(i < c.pieces ? T * c.cols : 0);
     f->row_scale = b.take<float>(T);
-    f->common = b.take<float>(64);
+    f->common = b.take<float>(1);
+    f->next = b.take<uint32_t>(c.pieces);
     f->hpart = b.take<float>(c.pieces > 1 || c.splits_h > 1 ? c.splits_h * T * D : 0);
     f->wpart = b.take<float>(c.splits_w > 1 ? static_cast<size_t>(c.splits_w) * c.cols * D : 0);
 }
@@ -854,9 +954,17 @@ int sm_count() {
     return sms;
 }
 
-// A 16-bit [rows, cols] matrix for loads of 128 rows x 64 K (K-major), or of 64 K x 64 columns (MN-major).
-int load_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld, bool mn) {
-    return make_tmap_2d_f16(m, base, rows, cols, ld, mn ? BK : kHalf, BK);
+// A 16-bit [rows, cols] matrix for loads of 128 x 128 elements as two panels of 64 columns (K-major: 128
+// rows, the columns are K; MN-major: 128 of K, the columns are M or N).  Where whole 64-column groups may be
+// read (cols a multiple of 64, or rows padded to one) a third dimension over the groups loads both panels
+// at once: one thread issues the copies, and with one per panel it was the bottleneck.
+int load_map(CUtensorMap* m, bool* whole, const void* base, int64_t rows, int64_t cols, int64_t ld) {
+    *whole = cols % 64 == 0;
+    if (!*whole) return make_tmap_2d_f16(m, base, rows, cols, ld, 128, 64);
+    const uint64_t dims[3] = {64, static_cast<uint64_t>(rows), static_cast<uint64_t>(cols / 64)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(ld) * 2, 128};
+    const uint32_t box[3] = {64, 128, 2};
+    return make_tmap(m, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 // Stores of 32 rows x 128 bytes: a 16-bit matrix, and fp32 slabs [slabs, rows, cols].
 int store_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld) {
@@ -878,8 +986,9 @@ int add_task(Launch* L, Task& t, int kind, bool a_mn, bool b_mn, int64_t M, int6
     t.N = static_cast<int>(N);
     t.tiles_m = static_cast<int>(ceil_div(M, kTile));
     t.tiles_n = static_cast<int>(ceil_div(N, kTile));
-    // 8 M tiles x about 9 N tiles at a time on 74 CTA pairs; a few N tiles run side by side
-    t.group = t.tiles_n <= 8 ? 1 : 8;
+    // 16 M tiles x about 5 N tiles at a time on 74 CTA pairs (8 x 9: 2 % slower); a few N tiles run side by side
+    t.group = t.tiles_n <= 8 ? 1 : 16;
+    t.K = static_cast<int>(K);
     t.k_blocks = static_cast<int>(ceil_div(K, BK));
     t.kb_per_split = static_cast<int>(ceil_div(t.k_blocks, splits));
     const int64_t before = L->tasks > 0 ? L->task[L->tasks - 1].items_end : 0;
@@ -959,8 +1068,8 @@ int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* h
         Launch L{};
         L.rows = r;
         Task t{};
-        MORPHO_TRY(load_map(&t.a, hidden, p->tokens, p->dim, ld_hidden(p), false));
-        MORPHO_TRY(load_map(&t.b, weight, p->vocab, p->dim, ld_weight(p), false));
+        MORPHO_TRY(load_map(&t.a, &t.a_whole, hidden, p->tokens, p->dim, ld_hidden(p)));
+        MORPHO_TRY(load_map(&t.b, &t.b_whole, weight, p->vocab, p->dim, ld_weight(p)));
         MORPHO_TRY(add_task(&L, t, kStats, false, false, p->tokens, p->vocab, p->dim, 1));
         MORPHO_TRY(launch<BF16>(dev, L, stream, "vocab_stats"));
     }
@@ -992,35 +1101,43 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
         if (i >= 0) L.rows.grad = nullptr;  // the first launch makes *common
         if (i >= 0) {
             const int v0 = i * c.cols;
-            const int64_t n = width(i);
+            const int64_t n = width(i), padded = ceil_div(n, 64) * 64;  // dz holds zeros up to whole panels
             Task w{}, h{};
             uint16_t* dw = static_cast<uint16_t*>(dweight) + static_cast<int64_t>(v0) * D;
-            MORPHO_TRY(load_map(&w.a, f.dz[i & 1], T, n, c.cols, true));
-            MORPHO_TRY(load_map(&w.b, hidden, T, D, ld_hidden(p), true));
+            MORPHO_TRY(load_map(&w.a, &w.a_whole, f.dz[i & 1], T, padded, c.cols));
+            MORPHO_TRY(load_map(&w.b, &w.b_whole, hidden, T, D, ld_hidden(p)));
             if (c.splits_w > 1)
                 MORPHO_TRY(slab_map(&w.out, f.wpart, c.splits_w, n, D));
             else
                 MORPHO_TRY(store_map(&w.out, dw, n, D, D));
-            MORPHO_TRY(add_task(&L, w, c.splits_w > 1 ? kPart : kOut, true, true, n, D, T, c.splits_w));
-            MORPHO_TRY(load_map(&h.a, f.dz[i & 1], T, n, c.cols, false));
-            MORPHO_TRY(load_map(&h.b, weight, p->vocab, D, ld_weight(p), true));
+            MORPHO_TRY(load_map(&h.a, &h.a_whole, f.dz[i & 1], T, padded, c.cols));
+            MORPHO_TRY(load_map(&h.b, &h.b_whole, weight, p->vocab, D, ld_weight(p)));
             h.b_row0 = v0;
             const bool direct = c.pieces == 1 && c.splits_h == 1;
-            // a shorter last piece may need fewer splits: their slabs keep the earlier pieces' sums
             if (direct)
                 MORPHO_TRY(store_map(&h.out, dhidden, T, D, D));
             else
                 MORPHO_TRY(slab_map(&h.out, f.hpart, c.splits_h, T, D));
-            MORPHO_TRY(add_task(&L, h, direct ? kOut : i == 0 ? kPart : kPartAdd, false, true, T, D, n,
-                                static_cast<int>(std::min<int64_t>(c.splits_h, ceil_div(n, BK)))));
+            // a shorter last piece may have fewer splits: the other slabs keep the earlier pieces' sums
+            const int splits_h = static_cast<int>(std::min<int64_t>(c.splits_h, ceil_div(n, BK)));
+            auto add_w = [&]() { return add_task(&L, w, c.splits_w > 1 ? kPart : kOut, true, true, n, D, T, c.splits_w); };
+            auto add_h = [&]() { return add_task(&L, h, direct ? kOut : i == 0 ? kPart : kPartAdd, false, true, T, D, n, splits_h); };
+            // the longest items first: the pairs that finish early take the short ones (dz last)
+            const bool h_first = ceil_div(n, splits_h) > ceil_div(T, c.splits_w);
+            MORPHO_TRY(h_first ? add_h() : add_w());
+            MORPHO_TRY(h_first ? add_w() : add_h());
+            L.next = f.next + i;
+        } else {
+            L.zero = f.next;
+            L.zeros = c.pieces;
         }
         if (i + 1 < c.pieces) {
             Task z{};
             z.v0 = (i + 1) * c.cols;
             z.b_row0 = z.v0;
-            MORPHO_TRY(load_map(&z.a, hidden, T, D, ld_hidden(p), false));
-            MORPHO_TRY(load_map(&z.b, weight, p->vocab, D, ld_weight(p), false));
-            MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, width(i + 1), c.cols));
+            MORPHO_TRY(load_map(&z.a, &z.a_whole, hidden, T, D, ld_hidden(p)));
+            MORPHO_TRY(load_map(&z.b, &z.b_whole, weight, p->vocab, D, ld_weight(p)));
+            MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, ceil_div(width(i + 1), 64) * 64, c.cols));
             MORPHO_TRY(add_task(&L, z, kDz, false, false, T, width(i + 1), D, 1));
         }
         MORPHO_TRY(launch<BF16>(dev, L, stream, i < 0 ? "vocab_dz" : "vocab_grad"));
