@@ -87,6 +87,26 @@ def test_rows(cuda, rows, residual):
     check(make(rows, 264, torch.float16, torch.float16, residual, seed=rows))
 
 
+# enough rows for the streaming kernels: every number of warps to a row, full and part-filled lanes
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,dim", [(4736, 8), (5001, 200), (4999, 256), (6000, 264), (4800, 512), (5003, 776), (4740, 1024),
+                                      (2400, 1032), (2501, 2048), (1300, 2056), (1201, 4096), (600, 4104), (700, 8192)])
+def test_many_rows(cuda, rows, dim, kind):
+    check(make(rows, dim, kind, kind, residual=True, seed=dim))
+    check(make(rows, dim, kind, torch.float32, residual=False, seed=dim))
+
+
+def test_many_strided_rows(cuda):
+    d = make(5000, 256, torch.float16, torch.float16, residual=True)
+    for k in ("x", "res", "gy", "gh"):
+        wide = torch.zeros(5000, 280, device="cuda", dtype=torch.float16)
+        wide[:, 8:264] = d[k]
+        d[k] = wide[:, 8:264]
+    check(d)
+    d["gy"] = d["gy"][:1].expand(5000, 256)
+    check(d)
+
+
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
 def test_fp32_weights(cuda, kind):
     check(make(77, 512, kind, torch.float32, residual=True))
