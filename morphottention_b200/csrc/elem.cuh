@@ -52,6 +52,40 @@ __device__ __forceinline__ float load_as_f32(const void* p, int type, int64_t i)
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+// N (4 or 8) consecutive elements of such a tensor from element i on, 16-byte aligned there if `whole`.
+template <int N>
+__device__ __forceinline__ void load_n_as_f32(const void* p, int type, int64_t i, bool whole, float* out) {
+    if (!whole) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) out[k] = load_as_f32(p, type, i + k);
+    } else if (type == MORPHO_DTYPE_F32) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k);
+            out[k] = x.x, out[k + 1] = x.y, out[k + 2] = x.z, out[k + 3] = x.w;
+        }
+    } else {
+        uint32_t u[N / 2];
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+        if (N == 8) {
+            const uint4 x = *reinterpret_cast<const uint4*>(q);
+            u[0] = x.x, u[1] = x.y, u[N / 2 - 2] = x.z, u[N / 2 - 1] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(q);
+            u[0] = x.x, u[1] = x.y;
+        }
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {
+            if (type == MORPHO_DTYPE_F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[k]));
+                out[2 * k] = f.x, out[2 * k + 1] = f.y;
+            } else {
+                out[2 * k] = __uint_as_float(u[k] << 16), out[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void store_from_f32(void* p, int type, int64_t i, float x) {
     if (type == MORPHO_DTYPE_F32)
         static_cast<float*>(p)[i] = x;

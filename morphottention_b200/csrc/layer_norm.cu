@@ -11,15 +11,16 @@
 // once.  The variance is the second moment about the mean just formed, which loses nothing to
 // cancellation.  All sums are fp32.
 //
-// Many rows (the *_stream kernels): a persistent CTA of eight warps, 1 to 8 of them to a row, a lane holding
-// up to 32 of its elements.  Each group of warps keeps a ring of rows in flight as bulk copies into shared
-// memory, so the bytes in flight do not depend on registers or occupancy, which the backward's dweight /
-// dbias sums (two fp32 registers per column, kept over all rows of the group) would otherwise limit.  The
-// CTA's groups join their sums in a fixed order and write one fp32 partial row per CTA; a second kernel
-// sums those in a fixed order (no atomics: the same bits every run).
-// Few rows, or rows that are not 16-byte aligned: a warp or a CTA loads its row into registers.  Rows longer
-// than a CTA's registers hold (dim > 8192) are read again from L2.
+// A group of threads (8 lanes to a CTA) holds its row in registers from the load to the store.  The forward
+// needs no more than that: with one row per group, many groups to an SM keep enough bytes in flight.
+// The backward is persistent: each group walks rows with the stride of the grid and keeps the dweight /
+// dbias sums of its columns in registers over all of them; the CTA's groups join theirs in a fixed order and
+// write one fp32 partial row per CTA, which a second kernel sums in a fixed order (no atomics: the same
+// bits every run).  Those sums, two fp32 registers per column, leave room for few warps, so above 256
+// columns the rows in flight are bulk copies into a ring in shared memory instead (the streaming kernel).
+// Rows longer than a CTA's registers hold (dim > 8192) are read again from L2.
 #include <algorithm>
+#include <initializer_list>
 
 #include "elem.cuh"
 #include "kernels.h"
@@ -28,15 +29,15 @@
 namespace morpho {
 namespace {
 
-constexpr int kCta = 256;        // threads per row of the CTA-wide kernels
-constexpr int kWarpsPerCta = 4;  // rows at a time of the warp-wide kernels
-constexpr int kMaxRegElems = 32; // row elements a thread holds
+constexpr int kCta = 256;       // threads of the kernels for any dim, and of the widest groups
+constexpr int kSmallCta = 128;  // threads of the other kernels
 
 constexpr uint32_t K_NORM = 7;   // kernel id in the device status word
 
 struct NormArgs {
     int64_t rows;
     int dim, wtype;
+    bool wvec;  // weight and bias start on 16-byte boundaries
     float eps;
     int64_t sx, sres, sgy, sgh;  // row strides in elements
     const void *x, *res, *w, *b; // forward inputs (x is h in the backward)
@@ -46,39 +47,60 @@ struct NormArgs {
     void* dx;
     float* part;  // [grid][2][dim] partial dweight / dbias
     uint32_t* status;
-    int stages;   // rows in flight per group of the streaming kernels
+    int stages;   // rows in flight per group of the streaming kernel
+    int mis;      // shifted rows: elements by which the tensors' bases miss a 16-byte boundary
 };
 
-// Sum of two values over the group; every thread gets the result.  GROUP 256 uses `scratch` (16
-// float2, used alternately by `turn`, so that one barrier per call suffices).
+// Threads of a CTA that works in groups of GROUP threads to a row.
+__host__ __device__ constexpr int cta_of(int group) { return group > kSmallCta ? group : kSmallCta; }
+
+// Sum of two values over the group; every thread of it gets the result.  Groups of more than a warp are the
+// whole CTA and use `scratch` (16 float2, used alternately by `turn`, so that one barrier per call suffices).
 template <int GROUP>
 __device__ __forceinline__ float2 group_sum(float a, float b, float2* scratch, int turn) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = (GROUP < 32 ? GROUP : 32) / 2; o > 0; o >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, o);
         b += __shfl_xor_sync(0xffffffffu, b, o);
     }
-    if (GROUP == 32) return make_float2(a, b);
-    const int warp = threadIdx.x >> 5;
+    if (GROUP <= 32) return make_float2(a, b);
     float2* s = scratch + (turn & 1) * 8;
-    if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
+    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = make_float2(a, b);
     __syncthreads();
-    float2 r = make_float2(0.f, 0.f);
+    float2 r = s[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 1; i < GROUP / 32; ++i) {
         r.x += s[i].x;
         r.y += s[i].y;
     }
     return r;
 }
 
-// NV packs of VEC elements per thread: pack i of thread l starts at column (i * GROUP + l) * VEC.
+// VEC elements of the weight or bias from column c on (`none` where there is none).
+template <int VEC>
+__device__ __forceinline__ void load_param(const void* p, const NormArgs& a, int c, float none, float* out) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out[k] = none;
+    } else if constexpr (VEC == 1) {
+        out[0] = load_as_f32(p, a.wtype, c);
+    } else {
+        load_n_as_f32<VEC>(p, a.wtype, c, a.wvec, out);
+    }
+}
+
+// NV packs of VEC elements per thread: pack i of thread l starts at column (i * GROUP + l) * VEC.  A CTA
+// has cta_of(GROUP) / GROUP rows; those past the end read the last row again and write nothing.
 template <class T, int VEC, int NV, int GROUP>
-__global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_norm_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(cta_of(GROUP)) layer_norm_fwd_kernel(const NormArgs a) {
     __shared__ float2 scratch[16];
-    const int l = GROUP == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t row = GROUP == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.rows) return;  // a whole warp, or never (GROUP 256)
+    pdl_release();
+    pdl_wait();
+    constexpr int ROWS = cta_of(GROUP) / GROUP;
+    const int l = threadIdx.x % GROUP;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / GROUP;
+    const bool live = at < a.rows;
+    const int64_t row = live ? at : a.rows - 1;
     const T* x = static_cast<const T*>(a.x) + row * a.sx;
     float v[NV * VEC];
     Pack<T, VEC> px[NV], pr[NV];
@@ -101,7 +123,7 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
             if (c >= a.dim) continue;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) px[i].v[k] = from_f32<T>(to_f32(px[i].v[k]) + to_f32(pr[i].v[k]));
-            store_pack<T, VEC>(h + c, px[i]);
+            if (live) store_pack<T, VEC>(h + c, px[i]);
         }
     }
     float sum = 0.f;
@@ -123,6 +145,7 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
             if ((i * GROUP + l) * VEC < a.dim) sq = fmaf(v[i * VEC + k], v[i * VEC + k], sq);
         }
     const float r = rsqrtf(group_sum<GROUP>(sq, 0.f, scratch, 1).x * inv + a.eps);
+    if (!live) return;
     if (l == 0) {
         a.mean[row] = mu;
         a.rstd[row] = r;
@@ -133,13 +156,112 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
         const int c = (i * GROUP + l) * VEC;
         if (c >= a.dim) continue;
         Pack<T, VEC> o;
+        float w[VEC], b[VEC];
+        load_param<VEC>(a.w, a, c, 1.f, w);
+        load_param<VEC>(a.b, a, c, 0.f, b);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const float w = a.w != nullptr ? load_as_f32(a.w, a.wtype, c + k) : 1.f;
-            const float b = a.b != nullptr ? load_as_f32(a.b, a.wtype, c + k) : 0.f;
-            o.v[k] = from_f32<T>(fmaf(v[i * VEC + k] * r, w, b));
-        }
+        for (int k = 0; k < VEC; ++k) o.v[k] = from_f32<T>(fmaf(v[i * VEC + k] * r, w[k], b[k]));
         store_pack<T, VEC>(y + c, o);
+    }
+}
+
+// ---- shifted rows: contiguous rows whose length is no multiple of 16 bytes ---------------------------------
+// All tensors are contiguous and miss a 16-byte boundary by the same number of elements, so a row begins
+// `off` elements into an aligned pack, in every tensor the same: packs are moved whole, the elements of the
+// first and the last that belong to the neighbours are masked, and only weight and bias are indexed by the
+// true column (from shared memory, one float in nine left out so that the lanes' strides hit all banks).
+
+template <int VEC>
+__device__ __forceinline__ int row_offset(const NormArgs& a, int64_t row) {
+    return (a.mis + static_cast<int>(row % VEC) * (a.dim % VEC)) % VEC;
+}
+
+__host__ __device__ constexpr int param_at(int c) { return c + 8 + ((c + 8) >> 3); }  // c >= -8
+
+template <int VEC, class T>
+__device__ __forceinline__ void store_cols(T* at, const Pack<T, VEC>& p, int col, int dim) {
+    if (col >= 0 && col + VEC <= dim) {
+        store_pack<T, VEC>(at, p);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (col + k >= 0 && col + k < dim) at[k] = p.v[k];
+    }
+}
+
+template <class T, int NV, int GROUP>
+__global__ void __launch_bounds__(cta_of(GROUP)) layer_norm_fwd_shift_kernel(const NormArgs a) {
+    constexpr int VEC = 16 / sizeof(T), ROWS = cta_of(GROUP) / GROUP;
+    extern __shared__ float ws[];  // weight, then bias
+    __shared__ float2 scratch[16];
+    pdl_release();
+    pdl_wait();
+    const int l = threadIdx.x % GROUP, g = threadIdx.x / GROUP;
+    const int width = param_at(a.dim + 8);
+    for (int c = static_cast<int>(threadIdx.x) - 8; c < a.dim + 8; c += cta_of(GROUP)) {
+        const bool in = c >= 0 && c < a.dim;
+        ws[param_at(c)] = a.w != nullptr && in ? load_as_f32(a.w, a.wtype, c) : 1.f;
+        ws[width + param_at(c)] = a.b != nullptr && in ? load_as_f32(a.b, a.wtype, c) : 0.f;
+    }
+    __syncthreads();
+    const float inv = 1.0f / static_cast<float>(a.dim);
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.rows; base += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const bool live = base + g < a.rows;
+        const int64_t row = live ? base + g : a.rows - 1;
+        const int off = row_offset<VEC>(a, row);
+        const int64_t at = row * a.dim - off;  // an aligned pack
+        Pack<T, VEC> px[NV], pr[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * GROUP + l) * VEC;
+            if (j - off < a.dim) {
+                px[i] = load_pack<T, VEC>(static_cast<const T*>(a.x) + at + j);
+                if (a.res != nullptr) pr[i] = load_pack<T, VEC>(static_cast<const T*>(a.res) + at + j);
+            }
+        }
+        float v[NV * VEC];
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * GROUP + l) * VEC, col = j - off;
+            if (a.res != nullptr && col < a.dim) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) px[i].v[k] = from_f32<T>(to_f32(px[i].v[k]) + to_f32(pr[i].v[k]));
+                if (live) store_cols<VEC>(static_cast<T*>(a.h) + at + j, px[i], col, a.dim);
+            }
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                v[i * VEC + k] = col + k >= 0 && col + k < a.dim ? to_f32(px[i].v[k]) : 0.f;
+                sum += v[i * VEC + k];
+            }
+        }
+        const float mu = group_sum<GROUP>(sum, 0.f, scratch, 0).x * inv;
+        float sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = (i * GROUP + l) * VEC - off;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                v[i * VEC + k] -= mu;
+                if (col + k >= 0 && col + k < a.dim) sq = fmaf(v[i * VEC + k], v[i * VEC + k], sq);
+            }
+        }
+        const float r = rsqrtf(group_sum<GROUP>(sq, 0.f, scratch, 1).x * inv + a.eps);
+        if (live && l == 0) {
+            a.mean[row] = mu;
+            a.rstd[row] = r;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * GROUP + l) * VEC, col = j - off;
+            if (col < a.dim && live) {
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    o.v[k] = from_f32<T>(fmaf(v[i * VEC + k] * r, ws[param_at(col + k)], ws[width + param_at(col + k)]));
+                store_cols<VEC>(static_cast<T*>(a.y) + at + j, o, col, a.dim);
+            }
+        }
     }
 }
 
@@ -181,19 +303,52 @@ __global__ void __launch_bounds__(kCta) layer_norm_fwd_long_kernel(const NormArg
     }
 }
 
+// The dweight / dbias sums of a CTA's GROUPS groups of G threads, each with NV packs of VEC columns a
+// thread, joined in the groups' order and written to `part` [2][dim].  Shared memory: sums_floats() floats.
+// Element (i, k) of thread l stands at (i VEC + k) (G + 1) + l, so that neither side conflicts on a bank.
+__host__ __device__ constexpr int sums_floats(int elems, int group, int groups) { return 2 * groups * elems * (group + 1); }
+
+// Column c of group i is element c + off(i) of its packs.
+template <int VEC, int NV, int G, int GROUPS, class Off>
+__device__ __forceinline__ void join_sums(float* sums, const float* dw, const float* db, int dim, float* part, Off off) {
+    constexpr int E = NV * VEC, SIZE = E * (G + 1);
+    const int l = threadIdx.x % G, g = threadIdx.x / G;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        sums[(2 * g) * SIZE + e * (G + 1) + l] = dw[e];
+        sums[(2 * g + 1) * SIZE + e * (G + 1) + l] = db[e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * dim; c += G * GROUPS) {
+        const int which = c >= dim, col = which ? c - dim : c;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const int e = col + off(i), k = e % VEC, t = e / VEC;
+            s += sums[(2 * i + which) * SIZE + ((t / G) * VEC + k) * (G + 1) + t % G];
+        }
+        part[c] = s;
+    }
+}
+
 template <class T, int VEC, int NV, int GROUP>
-__global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_norm_bwd_kernel(const NormArgs a) {
-    constexpr int E = NV * VEC;
+__global__ void __launch_bounds__(cta_of(GROUP), NV * VEC <= 8 && GROUP <= 32 ? 5 : 1) layer_norm_bwd_kernel(const NormArgs a) {
+    constexpr int E = NV * VEC, ROWS = cta_of(GROUP) / GROUP;
     __shared__ float2 scratch[16];
-    const int l = GROUP == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t first = GROUP == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerCta + (threadIdx.x >> 5) : blockIdx.x;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (GROUP == 32 ? kWarpsPerCta : 1);
+    extern __shared__ float sums[];
+    pdl_release();
+    pdl_wait();
+    const int l = threadIdx.x % GROUP, g = threadIdx.x / GROUP;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * ROWS;
     float dw[E], db[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.f;
     const float inv = 1.0f / static_cast<float>(a.dim);
     int turn = 0;
-    for (int64_t row = first; row < a.rows; row += step, ++turn) {
+    // the CTA's rows go together; those past the end read the last row again and add nothing
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * ROWS; base < a.rows; base += step, ++turn) {
+        const bool live = base + g < a.rows;
+        const int64_t row = live ? base + g : a.rows - 1;
         const T* h = static_cast<const T*>(a.x) + row * a.sx;
         const T* gy = static_cast<const T*>(a.gy) + row * a.sgy;
         const float mu = a.mean[row], r = a.rstd[row];
@@ -207,21 +362,23 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
             }
         }
         float s0 = 0.f, s1 = 0.f;
-        float xh[E], g[E];
+        float xh[E], gw[E];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * GROUP + l) * VEC;
             if (c < a.dim) {
+                float w[VEC];
+                load_param<VEC>(a.w, a, c, 1.f, w);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     const int e = i * VEC + k;
-                    const float d = to_f32(pg[i].v[k]);
+                    const float d = live ? to_f32(pg[i].v[k]) : 0.f;
                     xh[e] = (to_f32(ph[i].v[k]) - mu) * r;
-                    dw[e] = fmaf(d, xh[e], dw[e]);
+                    if (live) dw[e] = fmaf(d, xh[e], dw[e]);
                     db[e] += d;
-                    g[e] = a.w != nullptr ? d * load_as_f32(a.w, a.wtype, c + k) : d;
-                    s0 += g[e];
-                    s1 = fmaf(g[e], xh[e], s1);
+                    gw[e] = d * w[k];
+                    s0 += gw[e];
+                    s1 = fmaf(gw[e], xh[e], s1);
                 }
             }
         }
@@ -232,13 +389,13 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * GROUP + l) * VEC;
-            if (c >= a.dim) continue;
+            if (c >= a.dim || !live) continue;
             Pack<T, VEC> o, pd;
             if (gh != nullptr) pd = load_pack<T, VEC>(gh + c);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 const int e = i * VEC + k;
-                float d = r * (g[e] - mg - xh[e] * mgx);
+                float d = r * (gw[e] - mg - xh[e] * mgx);
                 if (gh != nullptr) d += to_f32(pd.v[k]);
                 o.v[k] = from_f32<T>(d);
             }
@@ -246,36 +403,7 @@ __global__ void __launch_bounds__(GROUP == 32 ? 32 * kWarpsPerCta : kCta) layer_
         }
     }
     if (a.part == nullptr) return;
-    float* part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
-    if (GROUP == 32) {
-        // the CTA's warps add their sums in turn (shared memory: one dweight and one dbias row)
-        extern __shared__ float rows[];
-        for (int w = 0; w < kWarpsPerCta; ++w) {
-            if ((threadIdx.x >> 5) == w) {
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) {
-                        const int c = (i * GROUP + l) * VEC + k;
-                        if (c >= a.dim) continue;
-                        rows[c] = w == 0 ? dw[i * VEC + k] : rows[c] + dw[i * VEC + k];
-                        rows[a.dim + c] = w == 0 ? db[i * VEC + k] : rows[a.dim + c] + db[i * VEC + k];
-                    }
-            }
-            __syncthreads();
-        }
-        for (int c = threadIdx.x; c < 2 * a.dim; c += 32 * kWarpsPerCta) part[c] = rows[c];
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const int c = (i * GROUP + l) * VEC + k;
-                if (c >= a.dim) continue;
-                part[c] = dw[i * VEC + k];
-                part[a.dim + c] = db[i * VEC + k];
-            }
-    }
+    join_sums<VEC, NV, GROUP, ROWS>(sums, dw, db, a.dim, a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.dim, [](int) { return 0; });
 }
 
 // Any dim: dx alone, one CTA per row, the row read twice.
@@ -324,7 +452,7 @@ __global__ void __launch_bounds__(kCta) layer_norm_bwd_cols_kernel(const NormArg
     part[a.dim + c] = db;
 }
 
-// ---- streaming kernels: aligned rows, up to 32 elements a lane ---------------------------------------
+// ---- the streaming backward: up to 32 elements a lane --------------------------------------------------
 
 constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = 32 * kStreamWarps;
@@ -357,14 +485,14 @@ struct RowRing {
     uint32_t row_bytes, stage_bytes;
     int stages;
 
-    // One thread: fetch row `row` of the given tensors (NULL: none) as use number i of the ring.
-    __device__ void fetch(int i, const void* a, const void* b, const void* c) const {
+    // One thread: fetch `bytes` of one row of the given tensors (c NULL: two) as use number i of the ring.
+    __device__ void fetch(int i, const void* a, const void* b, const void* c, uint32_t bytes) const {
         const int s = i % stages;
         const uint32_t bar = bars + 8 * s, dst = data + s * stage_bytes;
-        mbar_arrive_expect_tx(bar, row_bytes * (1 + (b != nullptr) + (c != nullptr)));
-        bulk_load(dst, a, row_bytes, bar);
-        if (b != nullptr) bulk_load(dst + row_bytes, b, row_bytes, bar);
-        if (c != nullptr) bulk_load(dst + 2 * row_bytes, c, row_bytes, bar);
+        mbar_arrive_expect_tx(bar, bytes * (2 + (c != nullptr)));
+        bulk_load(dst, a, bytes, bar);
+        bulk_load(dst + row_bytes, b, bytes, bar);
+        if (c != nullptr) bulk_load(dst + 2 * row_bytes, c, bytes, bar);
     }
     // After a wait for use i ran out: the copies that may still be in flight, each waited for in turn.
     __device__ void drain(int i, uint32_t* status) const {
@@ -380,6 +508,11 @@ template <class T>
 __device__ __forceinline__ Pack<T, 16 / sizeof(T)> shared_pack(uint32_t addr) {
     const uint4 x = ld_shared_u4(addr);
     return *reinterpret_cast<const Pack<T, 16 / sizeof(T)>*>(&x);
+}
+
+// Bytes of a row in the ring: shifted rows are fetched from the boundary before to the one after.
+__host__ __device__ constexpr int stream_row_bytes(int dim, int size, bool shift) {
+    return shift ? (dim + 2 * (16 / size) - 2) / (16 / size) * 16 : dim * size;
 }
 
 // Barriers and rings of the CTA's groups; every thread calls it.  Shared memory: rings, one after the other.
@@ -398,92 +531,9 @@ __device__ __forceinline__ RowRing make_ring(uint8_t* smem, uint64_t* bars, cons
     return r;
 }
 
-template <class T, int NV, int W>
-__global__ void __launch_bounds__(kStreamThreads, 2) layer_norm_fwd_stream_kernel(const NormArgs a) {
-    constexpr int VEC = 16 / sizeof(T), E = NV * VEC, G = 32 * W, GROUPS = kStreamWarps / W;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t bars[GROUPS * kMaxStages];
-    __shared__ float2 scratch[2][kStreamWarps];
-    pdl_release();
-    const int l = threadIdx.x % G, g = threadIdx.x / G;
-    const RowRing ring = make_ring<W>(smem, bars, a, a.dim * static_cast<int>(sizeof(T)), a.res != nullptr ? 2 : 1);
-    pdl_wait();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * GROUPS + g, step = static_cast<int64_t>(gridDim.x) * GROUPS;
-    const T *x = static_cast<const T*>(a.x), *res = static_cast<const T*>(a.res);
-    auto fetch = [&](int i, int64_t row) {
-        if (row < a.rows) ring.fetch(i, x + row * a.sx, res != nullptr ? res + row * a.sres : nullptr, nullptr);
-    };
-    if (l == 0)
-        for (int i = 0; i < a.stages; ++i) fetch(i, first + i * step);
-    float w[E], b[E];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const int c = (i * G + l) * VEC + k;
-            w[i * VEC + k] = a.w != nullptr && c < a.dim ? load_as_f32(a.w, a.wtype, c) : 1.f;
-            b[i * VEC + k] = a.b != nullptr && c < a.dim ? load_as_f32(a.b, a.wtype, c) : 0.f;
-        }
-    const float inv = 1.0f / static_cast<float>(a.dim);
-    int i = 0;
-    for (int64_t row = first; row < a.rows; row += step, ++i) {
-        if (!ring.wait(i, a.status, 1)) {
-            ring.drain(i, a.status);
-            break;
-        }
-        const uint32_t src = ring.stage(i);
-        float v[E];
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + l) * VEC;
-            if (c < a.dim) {
-                Pack<T, VEC> p = shared_pack<T>(src + c * sizeof(T));
-                if (res != nullptr) {
-                    const Pack<T, VEC> q = shared_pack<T>(src + ring.row_bytes + c * sizeof(T));
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) p.v[k] = from_f32<T>(to_f32(p.v[k]) + to_f32(q.v[k]));
-                    store_pack<T, VEC>(static_cast<T*>(a.h) + row * a.dim + c, p);
-                }
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    v[n * VEC + k] = to_f32(p.v[k]);
-                    sum += v[n * VEC + k];
-                }
-            }
-        }
-        const float mu = warps_sum<W>(sum, 0.f, scratch, 0, g).x * inv;
-        __syncwarp();
-        if (l == 0) fetch(i + a.stages, row + a.stages * step);  // the whole group has read the stage
-        float sq = 0.f;
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-            if ((n * G + l) * VEC < a.dim) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    v[n * VEC + k] -= mu;
-                    sq = fmaf(v[n * VEC + k], v[n * VEC + k], sq);
-                }
-            }
-        const float r = rsqrtf(warps_sum<W>(sq, 0.f, scratch, 1, g).x * inv + a.eps);
-        if (l == 0) {
-            a.mean[row] = mu;
-            a.rstd[row] = r;
-        }
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + l) * VEC;
-            if (c < a.dim) {
-                Pack<T, VEC> o;
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) o.v[k] = from_f32<T>(fmaf(v[n * VEC + k] * r, w[n * VEC + k], b[n * VEC + k]));
-                store_pack<T, VEC>(static_cast<T*>(a.y) + row * a.dim + c, o);
-            }
-        }
-    }
-}
-
-template <class T, int NV, int W>
+// SHIFT: shifted rows (above); the number of groups is then a multiple of VEC or covers the rows, so that
+// all rows of a group begin at one offset and its sums belong to the same columns throughout.
+template <class T, int NV, int W, bool SHIFT>
 __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 : 2) layer_norm_bwd_stream_kernel(const NormArgs a) {
     constexpr int VEC = 16 / sizeof(T), E = NV * VEC, G = 32 * W, GROUPS = kStreamWarps / W;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -492,17 +542,30 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
     pdl_release();
     const int l = threadIdx.x % G, g = threadIdx.x / G;
     const int tensors = a.gh != nullptr ? 3 : 2;
-    const RowRing ring = make_ring<W>(smem, bars, a, a.dim * static_cast<int>(sizeof(T)), tensors);
+    const RowRing ring = make_ring<W>(smem, bars, a, stream_row_bytes(a.dim, sizeof(T), SHIFT), tensors);
     float* ws = reinterpret_cast<float*>(smem + GROUPS * a.stages * ring.stage_bytes);  // the weight, fp32
     pdl_wait();
     const int64_t first = static_cast<int64_t>(blockIdx.x) * GROUPS + g, step = static_cast<int64_t>(gridDim.x) * GROUPS;
     const T *h = static_cast<const T*>(a.x), *gy = static_cast<const T*>(a.gy), *gh = static_cast<const T*>(a.gh);
+    const int off = SHIFT ? row_offset<VEC>(a, first) : 0;
+    const uint32_t bytes = SHIFT ? static_cast<uint32_t>((a.dim + off + VEC - 1) / VEC * 16) : ring.row_bytes;
     auto fetch = [&](int i, int64_t row) {
-        if (row < a.rows) ring.fetch(i, h + row * a.sx, gy + row * a.sgy, gh != nullptr ? gh + row * a.sgh : nullptr);
+        if (row < a.rows)
+            ring.fetch(i, h + row * a.sx - off, gy + row * a.sgy - off, gh != nullptr ? gh + row * a.sgh - off : nullptr, bytes);
     };
     if (l == 0)
         for (int i = 0; i < a.stages; ++i) fetch(i, first + i * step);
-    for (int c = threadIdx.x; c < a.dim; c += kStreamThreads) ws[c] = a.w != nullptr ? load_as_f32(a.w, a.wtype, c) : 1.f;
+    if (SHIFT) {
+        for (int c = static_cast<int>(threadIdx.x) - 8; c < a.dim + 8; c += kStreamThreads)
+            ws[param_at(c)] = a.w != nullptr && c >= 0 && c < a.dim ? load_as_f32(a.w, a.wtype, c) : 1.f;
+    } else {
+        for (int c = threadIdx.x * VEC; c < a.dim; c += kStreamThreads * VEC) {
+            float w[VEC];
+            load_param<VEC>(a.w, a, c, 1.f, w);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) ws[c + k] = w[k];
+        }
+    }
     __syncthreads();
     float dw[E], db[E];
 #pragma unroll
@@ -527,21 +590,27 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
         Pack<T, VEC> ph[NV];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + l) * VEC;
-            if (c < a.dim) {
+            const int c = (n * G + l) * VEC, col = c - off;
+            if (col < a.dim) {
                 const Pack<T, VEC> p = shared_pack<T>(src + c * sizeof(T)), q = shared_pack<T>(src + ring.row_bytes + c * sizeof(T));
                 if (gh != nullptr) ph[n] = shared_pack<T>(src + 2 * ring.row_bytes + c * sizeof(T));
                 float w[VEC];
+                if (SHIFT) {
 #pragma unroll
-                for (int k = 0; k < VEC; k += 4) {
-                    const float4 w4 = *reinterpret_cast<const float4*>(ws + c + k);
-                    w[k] = w4.x, w[k + 1] = w4.y, w[k + 2] = w4.z, w[k + 3] = w4.w;
+                    for (int k = 0; k < VEC; ++k) w[k] = ws[param_at(col + k)];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VEC; k += 4) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(ws + c + k);
+                        w[k] = w4.x, w[k + 1] = w4.y, w[k + 2] = w4.z, w[k + 3] = w4.w;
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
                     const int e = n * VEC + k;
-                    const float d = to_f32(q.v[k]);
-                    xh[e] = (to_f32(p.v[k]) - mu) * r;
+                    const bool in = !SHIFT || (col + k >= 0 && col + k < a.dim);
+                    const float d = in ? to_f32(q.v[k]) : 0.f;
+                    xh[e] = in ? (to_f32(p.v[k]) - mu) * r : 0.f;
                     dw[e] = fmaf(d, xh[e], dw[e]);
                     db[e] += d;
                     gw[e] = d * w[k];
@@ -556,8 +625,8 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
         const float mg = s.x * inv, mgx = s.y * inv;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int c = (n * G + l) * VEC;
-            if (c < a.dim) {
+            const int c = (n * G + l) * VEC, col = c - off;
+            if (col < a.dim) {
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) {
@@ -566,33 +635,20 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
                     if (gh != nullptr) d += to_f32(ph[n].v[k]);
                     o.v[k] = from_f32<T>(d);
                 }
-                store_pack<T, VEC>(static_cast<T*>(a.dx) + row * a.dim + c, o);
+                T* at = static_cast<T*>(a.dx) + row * a.dim + col;
+                if (SHIFT)
+                    store_cols<VEC>(at, o, col, a.dim);
+                else
+                    store_pack<T, VEC>(at, o);
             }
         }
         mu = mu1;
         r = r1;
     }
     if (a.part == nullptr) return;
-    // the groups add their sums in turn, over the rings (every fetched row has been waited for)
-    float* rows = reinterpret_cast<float*>(smem);
-    __syncthreads();
-    for (int t = 0; t < GROUPS; ++t) {
-        if (g == t) {
-#pragma unroll
-            for (int n = 0; n < NV; ++n)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) {
-                    const int c = (n * G + l) * VEC + k;
-                    if (c < a.dim) {
-                        rows[c] = t == 0 ? dw[n * VEC + k] : rows[c] + dw[n * VEC + k];
-                        rows[a.dim + c] = t == 0 ? db[n * VEC + k] : rows[a.dim + c] + db[n * VEC + k];
-                    }
-                }
-        }
-        __syncthreads();
-    }
-    float* part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
-    for (int c = threadIdx.x; c < 2 * a.dim; c += kStreamThreads) part[c] = rows[c];
+    __syncthreads();  // over the rings: every fetched row has been waited for
+    join_sums<VEC, NV, G, GROUPS>(reinterpret_cast<float*>(smem), dw, db, a.dim, a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.dim,
+                                  [&](int i) { return SHIFT ? row_offset<VEC>(a, static_cast<int64_t>(blockIdx.x) * GROUPS + i) : 0; });
 }
 
 // dweight / dbias = the sums of the `n` partial rows, in a fixed order: 32 columns per block, 32 threads a
@@ -658,29 +714,44 @@ NormArgs norm_args(const morpho_layer_norm_t* p) {
     return a;
 }
 
-// Calls f(VEC, NV, GROUP) as template constants for the width; false where the row is too long.
-// Vectors of 16 bytes where every row allows them, else single elements.  A warp takes rows of up to
-// 32 elements a lane, longer ones a CTA.
-template <int VEC, class F>
+// Calls f(NV, GROUP) as template constants for the width: groups of 8 or 16 lanes for rows that they hold
+// in 8 elements a lane, a warp for up to 32 elements a lane, then 128 and 256 threads of 16 or 32 in the
+// forward (65536 x 2048 bf16: 128 threads 6 TB/s, a warp with 64 elements a lane 5; the backward streams there).  Rows of single elements (VEC 1, unaligned) go to 256
+// threads above 256 columns: their many loads are better spread.  False where the row is too long.
+template <int VEC, bool FORWARD, class F>
 bool with_width(int dim, F f) {
-    constexpr int NV1 = VEC == 1 ? 8 : 8 / VEC;
-    auto fits = [&](int nv, int group) { return static_cast<int64_t>(nv) * VEC * group >= dim; };
-    if (fits(NV1, 32)) return f(std::integral_constant<int, NV1>(), std::integral_constant<int, 32>()), true;
-    if (fits(2 * NV1, 32)) return f(std::integral_constant<int, 2 * NV1>(), std::integral_constant<int, 32>()), true;
-    if (fits(4 * NV1, 32)) return f(std::integral_constant<int, 4 * NV1>(), std::integral_constant<int, 32>()), true;
-    if (fits(NV1, kCta)) return f(std::integral_constant<int, NV1>(), std::integral_constant<int, kCta>()), true;
-    if (fits(2 * NV1, kCta)) return f(std::integral_constant<int, 2 * NV1>(), std::integral_constant<int, kCta>()), true;
-    if (fits(4 * NV1, kCta)) return f(std::integral_constant<int, 4 * NV1>(), std::integral_constant<int, kCta>()), true;
+    using std::integral_constant;
+    constexpr int N = VEC == 1 ? 8 : 8 / VEC;  // packs of 8 elements
+#define MORPHO_TRY_WIDTH(packs, group) \
+    if (static_cast<int64_t>(packs) * VEC * (group) >= dim) return f(integral_constant<int, packs>(), integral_constant<int, group>()), true
+    MORPHO_TRY_WIDTH(N, 8);
+    MORPHO_TRY_WIDTH(N, 16);
+    MORPHO_TRY_WIDTH(N, 32);
+    if constexpr (VEC == 1) {
+        MORPHO_TRY_WIDTH(N, kCta);
+        MORPHO_TRY_WIDTH(2 * N, kCta);
+    } else {
+        MORPHO_TRY_WIDTH(2 * N, 32);
+        MORPHO_TRY_WIDTH(4 * N, 32);
+    }
+    if constexpr (FORWARD && VEC > 1) {
+        MORPHO_TRY_WIDTH(2 * N, kSmallCta);
+        MORPHO_TRY_WIDTH(4 * N, kSmallCta);
+    }
+    if constexpr (FORWARD || VEC == 1) MORPHO_TRY_WIDTH(4 * N, kCta);
+#undef MORPHO_TRY_WIDTH
     return false;
 }
-static_assert(kMaxRegElems == 32, "with_width covers 8, 16 and 32 elements a thread");
 
-// Calls f(NV, W) for the streaming kernels: up to 32 elements a lane, then 2, 4 and 8 warps to a row.
-template <int VEC, class F>
+// Calls f(NV, W) for the streaming backward: up to 32 elements a lane, then 2, 4 and 8 warps to a row.
+template <int VEC, bool SHIFT, class F>
 int with_stream(int dim, F f) {
     constexpr int NV1 = 8 / VEC;
     using std::integral_constant;
-    if (dim <= 256) return f(integral_constant<int, NV1>(), integral_constant<int, 1>());
+    if constexpr (SHIFT) {
+        dim += VEC - 1;
+        if (dim <= 256) return f(integral_constant<int, NV1>(), integral_constant<int, 1>());
+    }
     if (dim <= 512) return f(integral_constant<int, 2 * NV1>(), integral_constant<int, 1>());
     if (dim <= 1024) return f(integral_constant<int, 4 * NV1>(), integral_constant<int, 1>());
     if (dim <= 2048) return f(integral_constant<int, 4 * NV1>(), integral_constant<int, 2>());
@@ -688,23 +759,39 @@ int with_stream(int dim, F f) {
     return f(integral_constant<int, 4 * NV1>(), integral_constant<int, 8>());
 }
 
-constexpr int kStreamMaxDim = 8192;
+// How a call's rows lie: on 16-byte boundaries, shifted (contiguous, all tensors alike), or anyhow.
+enum class Rows { kAligned, kShifted, kAny };
 
-int stream_warps(int dim) { return dim <= 1024 ? 1 : dim <= 2048 ? 2 : dim <= 4096 ? 4 : 8; }
+constexpr int kMaxDim = 8192;                      // columns that registers hold
+constexpr int kShiftMaxDim = kMaxDim - 7;          // and with the widest offset
+constexpr int kStreamMinDim = 264;
 
-// Whether the rows are worth a ring: four for every group of one CTA per SM.
-bool streams(int64_t rows, int dim, bool vec, int sms) {
-    return vec && dim <= kStreamMaxDim && rows >= 4LL * sms * (kStreamWarps / stream_warps(dim));
+int stream_warps(int width) { return width <= 1024 ? 1 : width <= 2048 ? 2 : width <= 4096 ? 4 : 8; }
+
+// CTAs per SM of the streaming backward: its sums take too many registers for two above 512 columns.
+int stream_per_sm(int width) { return width <= 512 ? 2 : 1; }
+
+// Columns and the widest offset.
+int stream_width(int dim, Rows how, int type) { return dim + (how == Rows::kShifted ? 16 / dtype_bytes(type) - 1 : 0); }
+
+// Whether the backward streams: aligned rows up to 256 columns do not (a lane's eight sums leave room for so
+// many warps that plain loads do as well: 12608 x 256 fp16 11.7 us, not 11.5); above 1024 it always pays, in
+// between from one row for every group on (1184 x 1024: 7.4 us, not 8.5; with half the groups idle it loses).
+bool streams(int64_t rows, int dim, Rows how, int sms) {
+    if (how == Rows::kAny || dim > (how == Rows::kShifted ? kShiftMaxDim : kMaxDim)) return false;
+    if (how == Rows::kAligned && dim < kStreamMinDim) return false;
+    return dim > 1024 || rows >= static_cast<int64_t>(sms) * kStreamWarps;
 }
 
-// Launches a streaming kernel: `per_sm` CTAs on every SM, as many stages as fit beside `fixed` bytes.
+// Launches a streaming kernel: `per_sm` CTAs on every SM, as many stages as fit beside `fixed` bytes, `join`
+// bytes at the end.
 template <class K>
-int launch_stream(K kern, const DeviceInfo& dev, NormArgs& a, int type, int tensors, int fixed, int per_sm, int blocks, cudaStream_t stream) {
-    const int stage = a.dim * dtype_bytes(type) * tensors * (kStreamWarps / stream_warps(a.dim));
+int launch_stream(K kern, const DeviceInfo& dev, NormArgs& a, int row_bytes, int tensors, int groups, int fixed, int join, int per_sm, int blocks,
+                  cudaStream_t stream) {
+    const int stage = row_bytes * tensors * groups;
     const int room = (dev.smem_optin + 1024) / per_sm - 4096 - fixed;  // 4 KB: barriers, scratch, reserved
     a.stages = std::max(1, std::min(kMaxStages, room / stage));
-    // the joining of the groups' sums (two fp32 rows) lies over the rings
-    const int smem = std::max(a.stages * stage + fixed, 2 * a.dim * static_cast<int>(sizeof(float)));
+    const int smem = std::max(a.stages * stage + fixed, join);  // the joining of the groups' sums lies over the rings
     if (smem > dev.smem_optin - 2048) return set_error(MORPHO_ERR_INVALID, "layer norm: dim %d needs %d bytes of shared memory", a.dim, smem);
     MORPHO_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     MORPHO_CUDA_TRY(launch_after(kern, blocks, kStreamThreads, smem, stream, a));
@@ -712,60 +799,91 @@ int launch_stream(K kern, const DeviceInfo& dev, NormArgs& a, int type, int tens
 }
 
 template <class T>
-int forward_t(const DeviceInfo& dev, NormArgs a, int type, bool vec, cudaStream_t stream) {
+int forward_t(const DeviceInfo& dev, const NormArgs& a, Rows how, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     prof_begin(stream, "layer_norm_fwd");
-    if (streams(a.rows, a.dim, vec, dev.sms)) {
-        MORPHO_TRY(with_stream<V>(a.dim, [&](auto nv, auto w) {
-            return launch_stream(layer_norm_fwd_stream_kernel<T, decltype(nv)::value, decltype(w)::value>, dev, a, type, a.res != nullptr ? 2 : 1, 0, 2,
-                                 2 * dev.sms, stream);
-        }));
-        MORPHO_LAUNCH_CHECK("layer_norm_fwd");
-        return MORPHO_OK;
-    }
-    auto launch = [&](auto vecc, auto nv, auto group) {
-        constexpr int VEC = decltype(vecc)::value, NV = decltype(nv)::value, GROUP = decltype(group)::value;
-        const unsigned grid = GROUP == 32 ? (a.rows + kWarpsPerCta - 1) / kWarpsPerCta : a.rows;
-        layer_norm_fwd_kernel<T, VEC, NV, GROUP><<<grid, GROUP == 32 ? 32 * kWarpsPerCta : kCta, 0, stream>>>(a);
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto vecc) {
+        constexpr int VEC = decltype(vecc)::value;
+        return with_width<VEC, true>(a.dim, [&](auto nv, auto group) {
+            constexpr int NV = decltype(nv)::value, GROUP = decltype(group)::value;
+            const int64_t rows = cta_of(GROUP) / GROUP;
+            e = launch_after(layer_norm_fwd_kernel<T, VEC, NV, GROUP>, static_cast<unsigned>((a.rows + rows - 1) / rows), cta_of(GROUP), 0, stream, a);
+        });
     };
-    const bool done = vec ? with_width<V>(a.dim, [&](auto nv, auto g) { launch(std::integral_constant<int, V>(), nv, g); })
-                          : with_width<1>(a.dim, [&](auto nv, auto g) { launch(std::integral_constant<int, 1>(), nv, g); });
+    bool done;
+    // (a shifted kernel lays weight and bias out in shared memory first: for many rows)
+    if (how == Rows::kShifted && a.dim <= kShiftMaxDim && a.rows >= static_cast<int64_t>(dev.sms) * 8) {
+        done = with_width<V, true>(a.dim + V - 1, [&](auto nv, auto group) {
+            constexpr int NV = decltype(nv)::value, GROUP = decltype(group)::value;
+            const int64_t rows = cta_of(GROUP) / GROUP;
+            const int smem = 2 * param_at(a.dim + 8) * static_cast<int>(sizeof(float));
+            const int64_t most = static_cast<int64_t>(dev.sms) * std::max(1, std::min(4 * kSmallCta / cta_of(GROUP), 200 * 1024 / (smem + 1024)));
+            auto kern = layer_norm_fwd_shift_kernel<T, NV, GROUP>;
+            if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e == cudaSuccess) e = launch_after(kern, static_cast<unsigned>(std::min((a.rows + rows - 1) / rows, most)), cta_of(GROUP), smem, stream, a);
+        });
+    } else {
+        done = how == Rows::kAligned ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
+    }
     if (!done) layer_norm_fwd_long_kernel<T><<<static_cast<unsigned>(a.rows), kCta, 0, stream>>>(a);
+    MORPHO_CUDA_TRY(e);
     MORPHO_LAUNCH_CHECK("layer_norm_fwd");
     return MORPHO_OK;
 }
 
-// CTAs per SM of the streaming backward: its sums take too many registers for two above 512 columns.
-int bwd_per_sm(int dim) { return dim <= 512 ? 2 : 1; }
+// Partial rows (CTAs) of the backward: enough CTAs to fill the GPU, no more than the rows need.
+int bwd_blocks(int64_t rows, int dim, Rows how, int type, int sms) {
+    int64_t per, most;  // rows at a time of a CTA; CTAs
+    if (streams(rows, dim, how, sms)) {
+        const int width = stream_width(dim, how, type);
+        per = kStreamWarps / stream_warps(width);
+        most = stream_per_sm(width) * sms;
+        if (how == Rows::kShifted) most = std::max<int64_t>(8, most / 8 * 8);  // groups in multiples of a pack
+    } else if (dim <= 256) {
+        per = kSmallCta / (dim <= 64 ? 8 : dim <= 128 ? 16 : 32);
+        most = 5 * sms;
+    } else {
+        per = how == Rows::kAligned && dim <= 1024 ? kSmallCta / 32 : 1;
+        most = 2 * sms;
+    }
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, most)));
+}
 
-// Partial rows (CTAs) of the backward: enough CTAs to fill the GPU, no more than there are rows.
-int bwd_blocks(int64_t rows, int dim, bool stream, int sms) {
-    if (stream) return bwd_per_sm(dim) * sms;
-    const int64_t per = dim <= 32 * kMaxRegElems ? kWarpsPerCta : 1;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, 3 * sms)));
+template <class T, bool SHIFT>
+int backward_stream(const DeviceInfo& dev, NormArgs a, int type, int blocks, cudaStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const int width = stream_width(a.dim, SHIFT ? Rows::kShifted : Rows::kAligned, type);
+    return with_stream<V, SHIFT>(a.dim, [&](auto nv, auto w) {
+        constexpr int NV = decltype(nv)::value, W = decltype(w)::value;
+        const int join = a.part == nullptr ? 0 : static_cast<int>(sizeof(float)) * sums_floats(NV * V, 32 * W, kStreamWarps / W);
+        const int fixed = static_cast<int>(sizeof(float)) * (SHIFT ? param_at(a.dim + 8) : a.dim);
+        return launch_stream(layer_norm_bwd_stream_kernel<T, NV, W, SHIFT>, dev, a, stream_row_bytes(a.dim, sizeof(T), SHIFT), a.gh != nullptr ? 3 : 2,
+                             kStreamWarps / W, fixed, join, stream_per_sm(width), blocks, stream);
+    });
 }
 
 template <class T>
-int backward_t(const DeviceInfo& dev, NormArgs a, int type, bool vec, int blocks, cudaStream_t stream) {
+int backward_t(const DeviceInfo& dev, NormArgs a, int type, Rows how, int blocks, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     prof_begin(stream, "layer_norm_bwd");
-    if (streams(a.rows, a.dim, vec, dev.sms)) {
-        MORPHO_TRY(with_stream<V>(a.dim, [&](auto nv, auto w) {
-            return launch_stream(layer_norm_bwd_stream_kernel<T, decltype(nv)::value, decltype(w)::value>, dev, a, type, a.gh != nullptr ? 3 : 2,
-                                 a.dim * static_cast<int>(sizeof(float)), bwd_per_sm(a.dim), blocks, stream);
-        }));
+    if (streams(a.rows, a.dim, how, dev.sms)) {
+        MORPHO_TRY(how == Rows::kShifted ? (backward_stream<T, true>(dev, a, type, blocks, stream)) : (backward_stream<T, false>(dev, a, type, blocks, stream)));
         MORPHO_LAUNCH_CHECK("layer_norm_bwd");
         return MORPHO_OK;
     }
-    auto launch = [&](auto vecc, auto nv, auto group) {
-        constexpr int VEC = decltype(vecc)::value, NV = decltype(nv)::value, GROUP = decltype(group)::value;
-        const int smem = GROUP == 32 ? 2 * a.dim * static_cast<int>(sizeof(float)) : 0;
-        layer_norm_bwd_kernel<T, VEC, NV, GROUP>
-            <<<blocks, GROUP == 32 ? 32 * kWarpsPerCta : kCta, smem, stream>>>(a);
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto vecc) {
+        constexpr int VEC = decltype(vecc)::value;
+        return with_width<VEC, false>(a.dim, [&](auto nv, auto group) {
+            constexpr int NV = decltype(nv)::value, GROUP = decltype(group)::value;
+            constexpr int smem = sums_floats(NV * VEC, GROUP, cta_of(GROUP) / GROUP) * static_cast<int>(sizeof(float));
+            auto kern = layer_norm_bwd_kernel<T, VEC, NV, GROUP>;
+            if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e == cudaSuccess) e = launch_after(kern, static_cast<unsigned>(blocks), cta_of(GROUP), smem, stream, a);
+        });
     };
-    const bool done = vec ? with_width<V>(a.dim, [&](auto nv, auto g) { launch(std::integral_constant<int, V>(), nv, g); })
-                          : with_width<1>(a.dim, [&](auto nv, auto g) { launch(std::integral_constant<int, 1>(), nv, g); });
-    if (!done) {
+    if (!(how == Rows::kAligned ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>()))) {
         layer_norm_bwd_long_kernel<T><<<static_cast<unsigned>(a.rows), kCta, 0, stream>>>(a);
         if (a.part != nullptr) {
             count_launch();
@@ -773,8 +891,28 @@ int backward_t(const DeviceInfo& dev, NormArgs a, int type, bool vec, int blocks
             layer_norm_bwd_cols_kernel<T><<<grid, kCta, 0, stream>>>(a, (a.rows + blocks - 1) / blocks);
         }
     }
+    MORPHO_CUDA_TRY(e);
     MORPHO_LAUNCH_CHECK("layer_norm_bwd");
     return MORPHO_OK;
+}
+
+// How the rows of some tensors lie (base, row stride in elements; NULL: none); *mis for shifted ones.
+struct RowsOf {
+    const void* p;
+    int64_t stride;
+};
+Rows rows_of(std::initializer_list<RowsOf> tensors, int dim, int type, int* mis) {
+    const int size = dtype_bytes(type);
+    bool aligned = dim * size % 16 == 0, alike = true;
+    *mis = -1;
+    for (const RowsOf& t : tensors) {
+        if (t.p == nullptr) continue;
+        aligned = aligned && rows_aligned(t.p, t.stride, type);
+        const int m = static_cast<int>((reinterpret_cast<uintptr_t>(t.p) & 15u) / size);
+        alike = alike && t.stride == dim && (*mis < 0 || *mis == m);
+        *mis = m;
+    }
+    return aligned ? Rows::kAligned : alike ? Rows::kShifted : Rows::kAny;
 }
 
 int reduce_partials(const NormArgs& a, int n, void* dweight, void* dbias, cudaStream_t stream) {
@@ -819,16 +957,16 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_forward(const morpho_layer_nor
     a.res = residual;
     a.w = weight;
     a.b = bias;
+    a.wvec = aligned16(weight) && aligned16(bias);
     a.y = y;
     a.h = h;
     a.mean = mean;
     a.rstd = rstd;
-    const bool vec = p->dim * dtype_bytes(p->type) % 16 == 0 && rows_aligned(x, a.sx, p->type) &&
-                     rows_aligned(residual, a.sres, p->type) && aligned16(y) && (residual == nullptr || aligned16(h));
+    const Rows how = rows_of({{x, a.sx}, {residual, a.sres}, {y, a.dim}, {residual != nullptr ? h : nullptr, a.dim}}, p->dim, p->type, &a.mis);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p->type == MORPHO_DTYPE_F16) return forward_t<__half>(dev, a, p->type, vec, st);
-    if (p->type == MORPHO_DTYPE_BF16) return forward_t<__nv_bfloat16>(dev, a, p->type, vec, st);
-    return forward_t<float>(dev, a, p->type, vec, st);
+    if (p->type == MORPHO_DTYPE_F16) return forward_t<__half>(dev, a, how, st);
+    if (p->type == MORPHO_DTYPE_BF16) return forward_t<__nv_bfloat16>(dev, a, how, st);
+    return forward_t<float>(dev, a, how, st);
 }
 
 extern "C" MORPHO_API size_t morpho_sm100_layer_norm_backward_workspace_size(const morpho_layer_norm_t* p) {
@@ -837,7 +975,9 @@ extern "C" MORPHO_API size_t morpho_sm100_layer_norm_backward_workspace_size(con
     DeviceInfo dev;
     const int sms = current_device_info(&dev) == MORPHO_OK ? dev.sms : 148;
     clear_error();
-    return static_cast<size_t>(std::max(bwd_blocks(p->rows, p->dim, false, sms), bwd_blocks(p->rows, p->dim, true, sms))) * 2 * p->dim * sizeof(float) + 256;
+    int blocks = 0;
+    for (const Rows how : {Rows::kAligned, Rows::kShifted, Rows::kAny}) blocks = std::max(blocks, bwd_blocks(p->rows, p->dim, how, p->type, sms));
+    return static_cast<size_t>(blocks) * 2 * p->dim * sizeof(float) + 256;
 }
 
 extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_norm_t* p, const void* grad_y,
@@ -865,9 +1005,8 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
     DeviceInfo dev;
     MORPHO_TRY(current_device_info(&dev));
     NormArgs a = norm_args(p);
-    const bool vec = p->dim * dtype_bytes(p->type) % 16 == 0 && rows_aligned(h, a.sx, p->type) &&
-                     rows_aligned(grad_y, a.sgy, p->type) && rows_aligned(grad_h, a.sgh, p->type) && aligned16(dx);
-    const int blocks = bwd_blocks(p->rows, p->dim, streams(p->rows, p->dim, vec, dev.sms), dev.sms);
+    const Rows how = rows_of({{h, a.sx}, {grad_y, a.sgy}, {grad_h, a.sgh}, {dx, a.dim}}, p->dim, p->type, &a.mis);
+    const int blocks = bwd_blocks(p->rows, p->dim, how, p->type, dev.sms);
     const size_t need = static_cast<size_t>(blocks) * 2 * p->dim * sizeof(float);
     if (sums) {
         MORPHO_TRY(check_norm_ptr(workspace, "workspace", MORPHO_DTYPE_F32));
@@ -877,6 +1016,7 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
     a.status = dev.status;
     a.x = h;
     a.w = weight;
+    a.wvec = aligned16(weight);
     a.mean = const_cast<float*>(mean);
     a.rstd = const_cast<float*>(rstd);
     a.gy = grad_y;
@@ -885,11 +1025,11 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
     a.part = sums ? static_cast<float*>(workspace) : nullptr;
     int rc;
     if (p->type == MORPHO_DTYPE_F16)
-        rc = backward_t<__half>(dev, a, p->type, vec, blocks, st);
+        rc = backward_t<__half>(dev, a, p->type, how, blocks, st);
     else if (p->type == MORPHO_DTYPE_BF16)
-        rc = backward_t<__nv_bfloat16>(dev, a, p->type, vec, blocks, st);
+        rc = backward_t<__nv_bfloat16>(dev, a, p->type, how, blocks, st);
     else
-        rc = backward_t<float>(dev, a, p->type, vec, blocks, st);
+        rc = backward_t<float>(dev, a, p->type, how, blocks, st);
     if (rc != MORPHO_OK || !sums) return rc;
     return reduce_partials(a, blocks, dweight, dbias, st);
 }

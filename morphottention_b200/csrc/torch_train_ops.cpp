@@ -120,9 +120,9 @@ std::vector<at::Tensor> layer_norm_forward(const at::Tensor& x, const std::optio
         p.stride_residual = rr.stride;
     }
     auto y = at::empty(x.sizes(), x.options());
-    auto stats = at::empty({2, p.rows}, x.options().dtype(at::kFloat));
-    auto lead = x.sizes().slice(0, x.dim() - 1);
-    auto mean = stats.select(0, 0), rstd = stats.select(0, 1);
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    const auto f32 = x.options().dtype(at::kFloat);
+    auto mean = at::empty(lead, f32), rstd = at::empty(lead, f32);
     at::Tensor h;
     if (residual.has_value()) h = at::empty(x.sizes(), x.options());
     check_rc(morpho_sm100_layer_norm_forward(&p, xr.t.data_ptr(), residual.has_value() ? rr.t.data_ptr() : nullptr,
@@ -130,9 +130,8 @@ std::vector<at::Tensor> layer_norm_forward(const at::Tensor& x, const std::optio
                                              residual.has_value() ? h.data_ptr() : nullptr, mean.data_ptr<float>(),
                                              rstd.data_ptr<float>(), stream_of(x)),
              "layer_norm_forward");
-    std::vector<at::Tensor> out{y, mean.view(lead), rstd.view(lead)};
-    if (residual.has_value()) out.push_back(h);
-    return out;
+    if (residual.has_value()) return {y, mean, rstd, h};
+    return {y, mean, rstd};
 }
 
 std::vector<at::Tensor> layer_norm_backward(const at::Tensor& grad_y, const at::Tensor& h,

@@ -17,6 +17,11 @@ from ._ops import add_op_namespace_prefix, ops
 
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
+# the overloads themselves: a call through the packet looks them up every time
+_norm_forward, _norm_backward = ops.layer_norm_forward.default, ops.layer_norm_backward.default
+_loss_forward, _loss_backward = ops.linear_cross_entropy_forward.default, ops.linear_cross_entropy_backward.default
+_clip = ops.clip_grad_norm.default
+
 
 @torch.library.register_fake(add_op_namespace_prefix("layer_norm_forward"))
 def _layer_norm_forward_fake(x, weight, bias, eps, residual=None):
@@ -56,14 +61,14 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5, residual=No
     :param x: float16, bfloat16 or float32 CUDA tensor ``[..., dim]``; rows may have any common stride.
     :param weight, bias: ``[dim]`` in ``x``'s type or float32 (both in one), or None (a bias needs a weight).
     :returns: ``y`` and ``h`` contiguous in ``x``'s type, ``mean`` and ``rstd`` float32 ``[...]``."""
-    return ops.layer_norm_forward(x, weight, bias, eps, residual)
+    return _norm_forward(x, weight, bias, eps, residual)
 
 
 def layer_norm_backward(grad_y, h, weight, mean, rstd, grad_h=None):
     """``[dx, dweight, dbias]`` for the gradients of ``y`` and, with a residual, of ``h`` (``grad_h`` may be
     None).  ``dx`` is the gradient of the residual as well.  ``h`` is the forward's (``x`` without a
     residual).  Deterministic."""
-    return ops.layer_norm_backward(grad_y, h, weight, mean, rstd, grad_h)
+    return _norm_backward(grad_y, h, weight, mean, rstd, grad_h)
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -72,7 +77,7 @@ class LayerNormFunction(torch.autograd.Function):
         if not x.is_cuda:
             raise ValueError("layer_norm expects a CUDA tensor")
         ctx.set_materialize_grads(False)
-        y, mean, rstd, *h = ops.layer_norm_forward(x, weight, bias, eps, residual)
+        y, mean, rstd, *h = _norm_forward(x, weight, bias, eps, residual)
         ctx.save_for_backward(h[0] if h else x, weight, mean, rstd)
         ctx.has_bias = bias is not None
         ctx.has_residual = residual is not None
@@ -85,7 +90,7 @@ class LayerNormFunction(torch.autograd.Function):
             if grad_h is None:
                 return None, None, None, None, None
             return grad_h, None, None, None, grad_h if ctx.has_residual else None
-        dx, dw, db = ops.layer_norm_backward(grad_y, h, weight, mean, rstd, grad_h)
+        dx, dw, db = _norm_backward(grad_y, h, weight, mean, rstd, grad_h)
         return (dx, dw if weight is not None else None, db if ctx.has_bias else None, None,
                 dx if ctx.has_residual else None)
 
@@ -136,14 +141,14 @@ def linear_cross_entropy_forward(hidden, weight, target, ignore_index: int = -10
         loss NaN (no device assert).
     :param reduction: ``"none"`` (``[...]``), ``"sum"``, or ``"mean"`` over the tokens that are not
         ignored (0, not NaN, if all are)."""
-    return ops.linear_cross_entropy_forward(hidden, weight, target, ignore_index, _reduction(reduction))
+    return _loss_forward(hidden, weight, target, ignore_index, _reduction(reduction))
 
 
 def linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index: int = -100,
                                   reduction: str = "mean"):
     """``[dhidden, dweight]`` for the loss's float32 gradient (``target``'s shape for ``"none"``, else one
     element) and the forward's ``lse``.  Deterministic."""
-    return ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index,
+    return _loss_backward(grad_loss, hidden, weight, target, lse, ignore_index,
                                              _reduction(reduction))
 
 
@@ -152,7 +157,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     def forward(ctx, hidden, weight, target, ignore_index: int, reduction: int):
         if not hidden.is_cuda:
             raise ValueError("linear_cross_entropy expects CUDA tensors")
-        loss, lse = ops.linear_cross_entropy_forward(hidden, weight, target, ignore_index, reduction)
+        loss, lse = _loss_forward(hidden, weight, target, ignore_index, reduction)
         ctx.save_for_backward(hidden, weight, target, lse)
         ctx.options = ignore_index, reduction
         return loss
@@ -160,7 +165,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_loss):
         hidden, weight, target, lse = ctx.saved_tensors
-        dh, dw = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, *ctx.options)
+        dh, dw = _loss_backward(grad_loss, hidden, weight, target, lse, *ctx.options)
         return dh, dw, None, None, None
 
 
@@ -185,7 +190,7 @@ def clip_grad_norm(grads, max_norm: float, *, out=None, loss_scale: float = 1.0)
 
     A norm that is infinite or NaN makes the results non-finite."""
     grads = list(grads)
-    return ops.clip_grad_norm(grads, grads if out is None else list(out), max_norm, loss_scale)
+    return _clip(grads, grads if out is None else list(out), max_norm, loss_scale)
 
 
 def clip_grad_norm_(parameters, max_norm: float, *, loss_scale: float = 1.0) -> torch.Tensor:

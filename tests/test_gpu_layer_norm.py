@@ -96,6 +96,40 @@ def test_many_rows(cuda, rows, dim, kind):
     check(make(rows, dim, kind, torch.float32, residual=False, seed=dim))
 
 
+# rows whose length is no multiple of 16 bytes: every group width, and widths where the widest offset just
+# fits or needs the next group
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("rows,dim", [(5000, 3), (4999, 57), (5001, 63), (5003, 121), (4801, 249), (4805, 250), (4799, 507),
+                                      (5007, 777), (4741, 1001), (2500, 1017), (2501, 1019), (2399, 2045), (1301, 4091),
+                                      (1300, 6001), (1201, 8185), (1203, 8187)])
+def test_many_shifted_rows(cuda, rows, dim, kind):
+    check(make(rows, dim, kind, kind, residual=True, seed=dim))
+    check(make(rows, dim, kind, torch.float32, residual=False, seed=dim))
+
+
+@pytest.mark.parametrize("at", [1, 3])
+@pytest.mark.parametrize("dim", [256, 777])
+def test_contiguous_rows_off_a_boundary(cuda, at, dim):
+    """Contiguous inputs that begin inside a 16-byte pack: the backward's alike, the forward's unlike its outputs."""
+    d = make(5000, dim, torch.float16, torch.float16, residual=True)
+    for k in ("x", "res", "gy", "gh"):
+        flat = torch.full((5000 * dim + 8,), float("nan"), device="cuda", dtype=torch.float16)
+        flat[at:at + 5000 * dim] = d[k].flatten()
+        d[k] = flat[at:at + 5000 * dim].view(5000, dim)
+    check(d)
+
+
+def test_shifted_rows_do_not_see_their_neighbours(cuda):
+    d = make(5000, 777, torch.float16, torch.float16, residual=True)
+    y0, mean, rstd, h0 = M.layer_norm_forward(d["x"], d["w"], d["b"], EPS, d["res"])
+    dx0 = M.layer_norm_backward(d["gy"], h0, d["w"], mean, rstd, d["gh"])[0]
+    d["x"][1::2] = float("nan")
+    y, mean, rstd, h = M.layer_norm_forward(d["x"], d["w"], d["b"], EPS, d["res"])
+    assert torch.equal(y[::2], y0[::2]) and torch.equal(h[::2], h0[::2]) and y[1::2].isnan().all()
+    dx = M.layer_norm_backward(d["gy"], h, d["w"], mean, rstd, d["gh"])[0]
+    assert torch.equal(dx[::2], dx0[::2]) and dx[1::2].isnan().all()
+
+
 def test_many_strided_rows(cuda):
     d = make(5000, 256, torch.float16, torch.float16, residual=True)
     for k in ("x", "res", "gy", "gh"):
