@@ -7,9 +7,16 @@
 // it still holds.  A norm that is not finite makes the gradients non-finite (0 * inf, NaN), as dividing
 // by it does.
 //
-// The tensors are cut into chunks of kChunk elements, dealt to a persistent grid; the table of tensors
-// travels as a kernel parameter, so a launch needs no copy to the device and can be captured in a graph.
+// The tensors are cut into chunks, dealt to a persistent grid, of one 2 KB segment for each warp.  The table of tensors travels as a kernel parameter, so a launch needs no copy to the device
+// and can be captured in a graph.  (Taking the chunks in reverse in the second pass, to find in L2 what the
+// first read last, and storing with low cache priority changed nothing: 69 us each for 390 MB.)
+//
+// Alignment: a segment is read as the aligned 16-byte packs that cover it, with the neighbours' elements in
+// the first and the last masked.  Where input and output stand differently to a 16-byte boundary the
+// converted elements pass through shared memory, from which every aligned pack of the output is read as
+// two packs and shifted together; only a segment's first and last few elements are stored one by one.
 #include <algorithm>
+#include <type_traits>
 
 #include "elem.cuh"
 #include "kernels.h"
@@ -17,23 +24,41 @@
 namespace morpho {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kChunk = 8192;      // elements
-constexpr int kMaxBlocks = 1024;  // partial sums of one call
-constexpr int kTable = 768;       // tensors per launch: the parameter block stays under 32 KB
-
-struct Table {
-    int n, chunks;          // tensors; chunks in all
-    int chunk0[kTable + 1]; // first chunk of each tensor
-    const void* in[kTable];
-    void* out[kTable];
-    int64_t count[kTable];
-    uint8_t in_type[kTable], out_type[kTable];
+// A type of BYTES bytes (8 or 16) for one store.
+template <size_t BYTES>
+struct WordsOf {
+    using type = uint4;
 };
-static_assert(sizeof(Table) < 32000, "kernel parameter limit");
+template <>
+struct WordsOf<8> {
+    using type = uint2;
+};
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSegmentBytes = 2048;         // of one warp's input
+constexpr int kSumPerSm = 8, kScalePerSm = 5;  // CTAs per SM
+constexpr int kMaxBlocks = 2048;            // partial sums of one launch
+constexpr int kTable = 768;                 // tensors per launch: the parameter block stays under 32 KB
+constexpr int kFewTensors = 48, kSomeTensors = 192;  // smaller tables, cheaper to launch with
+
+template <int N>
+struct Table {
+    int n, chunks;      // tensors; chunks in all
+    int chunk0[N + 1];  // first chunk of each tensor
+    const void* in[N];
+    void* out[N];
+    int64_t count[N];
+    uint8_t in_type[N], out_type[N];
+};
+static_assert(sizeof(Table<kTable>) < 32000, "kernel parameter limit");
+
+__host__ __device__ constexpr int segment_of(int type) { return kSegmentBytes / dtype_bytes(type); }  // elements
+__host__ __device__ constexpr int chunk_of(int type) { return kWarps * segment_of(type); }
 
 // The tensor that chunk `c` belongs to (the last one whose first chunk is not after it).
-__device__ __forceinline__ int tensor_of(const Table& t, int c) {
+template <class Tab>
+__device__ __forceinline__ int tensor_of(const Tab& t, int c) {
     int lo = 0, hi = t.n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -56,73 +81,134 @@ __device__ __forceinline__ double block_sum(double x, double* scratch) {
     return r;
 }
 
-template <class T>
-__device__ __forceinline__ float chunk_squares(const T* p, int n) {
-    float s = 0.f;
-    constexpr int V = 16 / sizeof(T);
-    if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-        const int packs = n / V;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < packs; i += kThreads) {
-            const Pack<T, V> x = load_pack<T, V>(p + i * V);
+// f(pack, index of its first element) for the aligned packs of V elements that cover the warp's n elements
+// from p on, of which `off` elements of the first belong to what stands before p.  A whole segment on a
+// boundary has all its loads in flight at once.
+template <int V, class T, class F>
+__device__ __forceinline__ void each_pack(const T* p, int n, int off, F f) {
+    constexpr int PACKS = kSegmentBytes / (V * sizeof(T)) / 32;
+    const int lane = threadIdx.x & 31;
+    if (off == 0 && n == kSegmentBytes / static_cast<int>(sizeof(T))) {
+        Pack<T, V> x[PACKS];
 #pragma unroll
-            for (int k = 0; k < V; ++k) s = fmaf(to_f32(x.v[k]), to_f32(x.v[k]), s);
-        }
-        const int i = packs * V + threadIdx.x;
-        if (i < n) s = fmaf(to_f32(p[i]), to_f32(p[i]), s);
+        for (int i = 0; i < PACKS; ++i) x[i] = load_pack<T, V>(p + (i * 32 + lane) * V);
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) f(x[i], (i * 32 + lane) * V, std::true_type());
     } else {
-#pragma unroll 8
-        for (int i = threadIdx.x; i < n; i += kThreads) s = fmaf(to_f32(p[i]), to_f32(p[i]), s);
+#pragma unroll 2
+        for (int e = lane * V - off; e < n; e += 32 * V) f(load_pack<T, V>(p + e), e, std::false_type());
     }
+}
+
+template <class T>
+__device__ __forceinline__ float segment_squares(const T* p, int n) {
+    constexpr int V = 16 / sizeof(T);
+    float s = 0.f;
+    each_pack<V>(p, n, static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T)), [&](const auto& x, int e, auto whole) {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (whole || (e + k >= 0 && e + k < n)) s = fmaf(to_f32(x.v[k]), to_f32(x.v[k]), s);
+    });
     return s;
 }
 
-__global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Table t, double* part) {
-    __shared__ double scratch[kThreads / 32];
+template <class Tab>
+__global__ void __launch_bounds__(kThreads, kSumPerSm) grad_squares_kernel(const __grid_constant__ Tab t, double* part) {
+    __shared__ double scratch[kWarps];
+    pdl_release();
+    pdl_wait();
     double sum = 0.0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
         const int i = tensor_of(t, c);
-        const int64_t at = static_cast<int64_t>(c - t.chunk0[i]) * kChunk;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), t.count[i] - at));
+        const int64_t at = static_cast<int64_t>(c - t.chunk0[i]) * chunk_of(t.in_type[i]) + (threadIdx.x >> 5) * segment_of(t.in_type[i]);
+        const int n = static_cast<int>(min(static_cast<int64_t>(segment_of(t.in_type[i])), t.count[i] - at));
+        if (n <= 0) continue;
         const int type = t.in_type[i];
         if (type == MORPHO_DTYPE_F32)
-            sum += chunk_squares(static_cast<const float*>(t.in[i]) + at, n);
+            sum += segment_squares(static_cast<const float*>(t.in[i]) + at, n);
         else if (type == MORPHO_DTYPE_F16)
-            sum += chunk_squares(static_cast<const __half*>(t.in[i]) + at, n);
+            sum += segment_squares(static_cast<const __half*>(t.in[i]) + at, n);
         else
-            sum += chunk_squares(static_cast<const __nv_bfloat16*>(t.in[i]) + at, n);
+            sum += segment_squares(static_cast<const __nv_bfloat16*>(t.in[i]) + at, n);
     }
     sum = block_sum(sum, scratch);
     if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
 
-template <class T, class O>
-__device__ __forceinline__ void chunk_scale(const T* p, O* q, int n, float by) {
-    constexpr int V = 16 / (sizeof(T) > sizeof(O) ? sizeof(T) : sizeof(O));
-    const bool whole = reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) == 0 &&
-                       reinterpret_cast<uintptr_t>(q) % (V * sizeof(O)) == 0;
-    if (whole) {
-        const int packs = n / V;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < packs; i += kThreads) {
-            const Pack<T, V> x = load_pack<T, V>(p + i * V);
-            Pack<O, V> y;
+// Four words of the 32 bytes a | b from byte `shift` (0..15) on.
+__device__ __forceinline__ uint4 shift_packs(uint4 a, uint4 b, int shift) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (shift & 8) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) y.v[k] = from_f32<O>(to_f32(x.v[k]) * by);
-            store_pack<O, V>(q + i * V, y);
-        }
-        const int i = packs * V + threadIdx.x;
-        if (i < n) q[i] = from_f32<O>(to_f32(p[i]) * by);
-    } else {
-#pragma unroll 8
-        for (int i = threadIdx.x; i < n; i += kThreads) q[i] = from_f32<O>(to_f32(p[i]) * by);
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
     }
+    if (shift & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    const int bits = (shift & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__global__ void __launch_bounds__(kThreads)
-    grad_scale_kernel(const __grid_constant__ Table t, const double* part, int parts, float max_norm, float inv_scale,
+// q[0..n) = by * p[0..n) of one warp; `stage`: its shared memory, kStageBytes.
+constexpr int kStageBytes = (segment_of(MORPHO_DTYPE_F16) + 16) * 4;
+
+template <class T, class O>
+__device__ __forceinline__ void segment_scale(const T* p, O* q, int n, float by, uint8_t* stage) {
+    // as many elements as both sides move at once, so that a warp's stores cover whole sectors too
+    constexpr int VO = 16 / sizeof(O), V = sizeof(T) > sizeof(O) ? 16 / sizeof(T) : VO;
+    using Words = typename WordsOf<V * sizeof(O)>::type;
+    const int lane = threadIdx.x & 31;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) % (V * sizeof(T)) / sizeof(T));
+    const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(q) & 15u) / sizeof(O));
+    auto scaled = [&](const auto& x) {
+        Pack<O, V> y;
+#pragma unroll
+        for (int k = 0; k < V; ++k) y.v[k] = from_f32<O>(to_f32(x.v[k]) * by);
+        return y;
+    };
+    if (mis % V == off) {  // packs fall on packs
+        each_pack<V>(p, n, off, [&](const auto& x, int e, auto whole) {
+            const Pack<O, V> y = scaled(x);
+            if (whole || (e >= 0 && e + V <= n)) {
+                *reinterpret_cast<Words*>(q + e) = *reinterpret_cast<const Words*>(y.v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k)
+                    if (e + k >= 0 && e + k < n) q[e + k] = y.v[k];
+            }
+        });
+        return;
+    }
+    __syncwarp();  // the previous segment's packs have been read
+    each_pack<V>(p, n, off, [&](const auto& x, int e, auto) {
+        const Pack<O, V> y = scaled(x);
+        *reinterpret_cast<Words*>(reinterpret_cast<O*>(stage) + e + off) = *reinterpret_cast<const Words*>(y.v);
+    });
+    __syncwarp();
+    const int head = min(n, mis == 0 ? 0 : VO - mis);  // elements before q's first aligned pack
+    const int packs = (n - head) / VO, tail = head + packs * VO;
+    const O* from = reinterpret_cast<const O*>(stage) + off;
+    const int byte0 = (off + head) * static_cast<int>(sizeof(O));
+#pragma unroll 2
+    for (int i = lane; i < packs; i += 32) {
+        const uint4* a = reinterpret_cast<const uint4*>(stage) + (byte0 >> 4) + i;
+        reinterpret_cast<uint4*>(q + head)[i] = shift_packs(a[0], a[1], byte0 & 15);
+    }
+    if (lane < head) q[lane] = from[lane];
+    if (tail + lane < n) q[tail + lane] = from[tail + lane];
+}
+
+template <class Tab>
+__global__ void __launch_bounds__(kThreads, kScalePerSm)
+    grad_scale_kernel(const __grid_constant__ Tab t, const double* part, int parts, float max_norm, float inv_scale,
                       float* norm_out) {
-    __shared__ double scratch[kThreads / 32];
+    extern __shared__ __align__(16) uint8_t stages[];
+    __shared__ double scratch[kWarps];
+    pdl_release();
+    pdl_wait();
     double sum = 0.0;
     for (int i = threadIdx.x; i < parts; i += kThreads) sum += part[i];
     sum = block_sum(sum, scratch);
@@ -131,18 +217,19 @@ __global__ void __launch_bounds__(kThreads)
     c = c > 1.0f ? 1.0f : c;  // NaN stays NaN
     if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
     const float by = c * inv_scale;
+    uint8_t* stage = stages + (threadIdx.x >> 5) * kStageBytes;
     for (int k = blockIdx.x; k < t.chunks; k += gridDim.x) {
         const int i = tensor_of(t, k);
-        const int64_t at = static_cast<int64_t>(k - t.chunk0[i]) * kChunk;
-        const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), t.count[i] - at));
-        if (by == 1.0f && t.in[i] == t.out[i]) continue;  // in place and nothing to change
+        const int64_t at = static_cast<int64_t>(k - t.chunk0[i]) * chunk_of(t.in_type[i]) + (threadIdx.x >> 5) * segment_of(t.in_type[i]);
+        const int n = static_cast<int>(min(static_cast<int64_t>(segment_of(t.in_type[i])), t.count[i] - at));
+        if (n <= 0 || (by == 1.0f && t.in[i] == t.out[i])) continue;  // in place and nothing to change
         auto out = [&](auto* p) {
             if (t.out_type[i] == MORPHO_DTYPE_F32)
-                chunk_scale(p + at, static_cast<float*>(t.out[i]) + at, n, by);
+                segment_scale(p + at, static_cast<float*>(t.out[i]) + at, n, by, stage);
             else if (t.out_type[i] == MORPHO_DTYPE_F16)
-                chunk_scale(p + at, static_cast<__half*>(t.out[i]) + at, n, by);
+                segment_scale(p + at, static_cast<__half*>(t.out[i]) + at, n, by, stage);
             else
-                chunk_scale(p + at, static_cast<__nv_bfloat16*>(t.out[i]) + at, n, by);
+                segment_scale(p + at, static_cast<__nv_bfloat16*>(t.out[i]) + at, n, by, stage);
         };
         if (t.in_type[i] == MORPHO_DTYPE_F32)
             out(static_cast<const float*>(t.in[i]));
@@ -154,12 +241,13 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Fills the table from tensor `first` on; returns the tensor after the last one taken.
-int64_t fill(Table* t, const morpho_tensor_pair_t* pairs, int64_t first, int64_t count) {
+template <int N>
+int64_t fill(Table<N>* t, const morpho_tensor_pair_t* pairs, int64_t first, int64_t count) {
     t->n = 0;
     int64_t chunks = 0, i = first;
-    for (; i < count && t->n < kTable; ++i) {
+    for (; i < count && t->n < N; ++i) {
         if (pairs[i].count == 0) continue;
-        const int64_t more = (pairs[i].count + kChunk - 1) / kChunk;
+        const int64_t more = (pairs[i].count + chunk_of(pairs[i].in_type) - 1) / chunk_of(pairs[i].in_type);
         if (chunks + more > (1LL << 30)) break;
         const int k = t->n++;
         t->chunk0[k] = static_cast<int>(chunks);
@@ -175,18 +263,34 @@ int64_t fill(Table* t, const morpho_tensor_pair_t* pairs, int64_t first, int64_t
     return i;
 }
 
-int launch_squares(const Table& t, double* part, int blocks, cudaStream_t stream) {
-    prof_begin(stream, "grad_squares");
-    grad_squares_kernel<<<blocks, kThreads, 0, stream>>>(t, part);
-    MORPHO_LAUNCH_CHECK("grad_squares");
-    return MORPHO_OK;
-}
-
-int launch_scale(const Table& t, const double* part, int parts, float max_norm, float inv_scale, float* norm, int blocks,
-                 cudaStream_t stream) {
-    prof_begin(stream, "grad_scale");
-    grad_scale_kernel<<<blocks, kThreads, 0, stream>>>(t, part, parts, max_norm, inv_scale, norm);
-    MORPHO_LAUNCH_CHECK("grad_scale");
+// Both passes, with tables of up to N tensors.
+template <int N>
+int clip(const DeviceInfo& dev, const morpho_tensor_pair_t* pairs, int64_t count, float max_norm, float inv_scale, float* norm, double* part,
+         int64_t limit, cudaStream_t stream) {
+    auto scale = grad_scale_kernel<Table<N>>;
+    constexpr int smem = kWarps * kStageBytes;
+    static_assert(smem <= 48 * 1024, "shared memory");
+    Table<N> t;
+    int launches = 0;
+    int64_t parts = 0, i = 0;
+    do {
+        i = fill(&t, pairs, i, count);
+        const int blocks = std::max(1, std::min({t.chunks, kSumPerSm * dev.sms, kMaxBlocks}));
+        if (parts + blocks > limit) return set_error(MORPHO_ERR_WORKSPACE, "clip: too many elements for one call");
+        prof_begin(stream, "grad_squares");
+        MORPHO_CUDA_TRY(launch_after(grad_squares_kernel<Table<N>>, blocks, kThreads, 0, stream, t, part + parts));
+        MORPHO_LAUNCH_CHECK("grad_squares");
+        parts += blocks;
+        ++launches;
+    } while (i < count);
+    i = 0;
+    for (int k = 0; k < launches; ++k) {
+        if (launches > 1) i = fill(&t, pairs, i, count);
+        const int blocks = std::max(1, std::min(t.chunks, kScalePerSm * dev.sms));
+        prof_begin(stream, "grad_scale");
+        MORPHO_CUDA_TRY(launch_after(scale, blocks, kThreads, smem, stream, t, part, static_cast<int>(parts), max_norm, inv_scale, k == 0 ? norm : nullptr));
+        MORPHO_LAUNCH_CHECK("grad_scale");
+    }
     return MORPHO_OK;
 }
 
@@ -237,24 +341,8 @@ extern "C" MORPHO_API int morpho_sm100_clip_grad_norm(const morpho_tensor_pair_t
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* part = static_cast<double*>(workspace);
     const float inv_scale = 1.0f / loss_scale;
-    const int most = std::min(4 * dev.sms, kMaxBlocks);
     const int64_t limit = static_cast<int64_t>(workspace_bytes / sizeof(double));
-    Table t;
-    int launches = 0;
-    int64_t parts = 0, i = 0;
-    do {
-        i = fill(&t, pairs, i, count);
-        const int blocks = std::max(1, std::min(t.chunks, most));
-        if (parts + blocks > limit) return set_error(MORPHO_ERR_WORKSPACE, "clip: too many elements for one call");
-        MORPHO_TRY(launch_squares(t, part + parts, blocks, st));
-        parts += blocks;
-        ++launches;
-    } while (i < count);
-    i = 0;
-    for (int k = 0; k < launches; ++k) {
-        if (launches > 1) i = fill(&t, pairs, i, count);
-        const int blocks = std::max(1, std::min(t.chunks, most));
-        MORPHO_TRY(launch_scale(t, part, static_cast<int>(parts), max_norm, inv_scale, k == 0 ? norm : nullptr, blocks, st));
-    }
-    return MORPHO_OK;
+    return count <= kFewTensors    ? clip<kFewTensors>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st)
+           : count <= kSomeTensors ? clip<kSomeTensors>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st)
+                                   : clip<kTable>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st);
 }
