@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/morpho_sm100.h"
 
 namespace morpho {
@@ -56,6 +58,19 @@ int prof_collect(char* names, int name_len, float* total_ms, int* counts, int ma
         ::morpho::count_launch();                                                                              \
         ::morpho::prof_end(name, stream);                                                                      \
     } while (0)
+
+// Allow a kernel `bytes` of dynamic shared memory on the current device (one `set` per kernel: the call is
+// made when a device's first launch, or a larger one, needs it).
+struct SharedLimit {
+    std::atomic<int> set[64] = {};
+    template <class K>
+    cudaError_t raise(K kernel, int device, int bytes) {
+        if (bytes <= 48 * 1024 || set[device].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) set[device].store(bytes, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 // Launch a kernel that begins with pdl_wait(): its CTAs may be set up while the kernel before it on the
 // stream drains (programmatic stream serialization), instead of after it has ended.

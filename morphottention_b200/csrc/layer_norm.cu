@@ -786,14 +786,14 @@ bool streams(int64_t rows, int dim, Rows how, int sms) {
 // Launches a streaming kernel: `per_sm` CTAs on every SM, as many stages as fit beside `fixed` bytes, `join`
 // bytes at the end.
 template <class K>
-int launch_stream(K kern, const DeviceInfo& dev, NormArgs& a, int row_bytes, int tensors, int groups, int fixed, int join, int per_sm, int blocks,
+int launch_stream(K kern, SharedLimit& limit, const DeviceInfo& dev, NormArgs& a, int row_bytes, int tensors, int groups, int fixed, int join, int per_sm, int blocks,
                   cudaStream_t stream) {
     const int stage = row_bytes * tensors * groups;
     const int room = (dev.smem_optin + 1024) / per_sm - 4096 - fixed;  // 4 KB: barriers, scratch, reserved
     a.stages = std::max(1, std::min(kMaxStages, room / stage));
     const int smem = std::max(a.stages * stage + fixed, join);  // the joining of the groups' sums lies over the rings
     if (smem > dev.smem_optin - 2048) return set_error(MORPHO_ERR_INVALID, "layer norm: dim %d needs %d bytes of shared memory", a.dim, smem);
-    MORPHO_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MORPHO_CUDA_TRY(limit.raise(kern, dev.device, smem));
     MORPHO_CUDA_TRY(launch_after(kern, blocks, kStreamThreads, smem, stream, a));
     return MORPHO_OK;
 }
@@ -820,7 +820,8 @@ int forward_t(const DeviceInfo& dev, const NormArgs& a, Rows how, cudaStream_t s
             const int smem = 2 * param_at(a.dim + 8) * static_cast<int>(sizeof(float));
             const int64_t most = static_cast<int64_t>(dev.sms) * std::max(1, std::min(4 * kSmallCta / cta_of(GROUP), 200 * 1024 / (smem + 1024)));
             auto kern = layer_norm_fwd_shift_kernel<T, NV, GROUP>;
-            if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            static SharedLimit limit;
+            e = limit.raise(kern, dev.device, smem);
             if (e == cudaSuccess) e = launch_after(kern, static_cast<unsigned>(std::min((a.rows + rows - 1) / rows, most)), cta_of(GROUP), smem, stream, a);
         });
     } else {
@@ -858,7 +859,8 @@ int backward_stream(const DeviceInfo& dev, NormArgs a, int type, int blocks, cud
         constexpr int NV = decltype(nv)::value, W = decltype(w)::value;
         const int join = a.part == nullptr ? 0 : static_cast<int>(sizeof(float)) * sums_floats(NV * V, 32 * W, kStreamWarps / W);
         const int fixed = static_cast<int>(sizeof(float)) * (SHIFT ? param_at(a.dim + 8) : a.dim);
-        return launch_stream(layer_norm_bwd_stream_kernel<T, NV, W, SHIFT>, dev, a, stream_row_bytes(a.dim, sizeof(T), SHIFT), a.gh != nullptr ? 3 : 2,
+        static SharedLimit limit;
+        return launch_stream(layer_norm_bwd_stream_kernel<T, NV, W, SHIFT>, limit, dev, a, stream_row_bytes(a.dim, sizeof(T), SHIFT), a.gh != nullptr ? 3 : 2,
                              kStreamWarps / W, fixed, join, stream_per_sm(width), blocks, stream);
     });
 }
@@ -879,7 +881,8 @@ int backward_t(const DeviceInfo& dev, NormArgs a, int type, Rows how, int blocks
             constexpr int NV = decltype(nv)::value, GROUP = decltype(group)::value;
             constexpr int smem = sums_floats(NV * VEC, GROUP, cta_of(GROUP) / GROUP) * static_cast<int>(sizeof(float));
             auto kern = layer_norm_bwd_kernel<T, VEC, NV, GROUP>;
-            if (smem > 48 * 1024) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            static SharedLimit limit;
+            e = limit.raise(kern, dev.device, smem);
             if (e == cudaSuccess) e = launch_after(kern, static_cast<unsigned>(blocks), cta_of(GROUP), smem, stream, a);
         });
     };

@@ -22,6 +22,7 @@
 // MMA issuer (rank 0 of the pair), warps 2-9 epilogue, warp 10 scheduler; the accumulator is double-buffered in TMEM, and
 // results leave through TMA stores from a swizzled box per warp.
 #include <algorithm>
+#include <type_traits>
 
 #include "elem.cuh"
 #include "kernels.h"
@@ -596,9 +597,11 @@ __global__ void __launch_bounds__(256) vocab_finish_kernel(const float* part, in
 
 // ---- a few tokens: logits on CUDA cores ------------------------------------------------------------
 
-constexpr int kFewTokens = 4;
-constexpr int kFewThreads = 256;
-constexpr int kFewRows = 4;  // vocabulary rows a warp reads at a time
+constexpr int kFewTokens = 8;
+constexpr int kFewWarps = 8;
+constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kFewMaxStages = 6, kFewRing = 192 * 1024;
+constexpr int kFewMaxDim = 6144;  // two stages for every warp in the ring
 
 // (m, s) <- (m, s) joined with (om, os): m the maximum, s the sum of exp(z - m).
 __device__ __forceinline__ void join(float& m, float& s, float om, float os) {
@@ -627,18 +630,46 @@ __device__ __forceinline__ void unpack8(uint4 x, float* f) {
     }
 }
 
-// Up to TT tokens against the whole vocabulary, bound by reading the weight once: each warp takes a
-// contiguous range of its rows, kFewRows at a time, the hidden rows stand in shared memory, and every
-// CTA leaves one piece of each token's statistics.
-template <bool BF16, int TT>
-__global__ void __launch_bounds__(kFewThreads) vocab_few_kernel(const Rowwise p, const uint16_t* hidden, int64_t ldh,
-                                                                const uint16_t* weight, int64_t ldw, int D) {
-    extern __shared__ uint4 hs[];  // [TT][D / 8]
-    __shared__ float2 sh[kFewThreads / 32][TT];
+// Up to TT tokens against the whole vocabulary, bound by reading the weight once.  Each warp streams a
+// contiguous range of rows through a ring of its own in shared memory (bulk copies of 32 / GL rows), so the
+// bytes in flight do not hang on registers; GL lanes share a row, the groups of a warp work on as many rows,
+// each keeping the running maximum and sum of its own.  The hidden rows stand in shared memory too, and every
+// CTA (one per SM) leaves one piece of each token's statistics.
+template <bool BF16, int TT, int GL>
+__global__ void __launch_bounds__(kFewThreads, 1) vocab_few_kernel(const Rowwise p, const uint16_t* hidden, int64_t ldh, const uint16_t* weight,
+                                                                   int64_t ldw, int D, int stages, uint32_t* status) {
+    constexpr int ROWS = 32 / GL;  // at a time
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint64_t bars[kFewWarps * kFewMaxStages];
+    __shared__ float2 sh[kFewWarps][TT];
+    const int lane = threadIdx.x & 31, warp = warp_id(), l = lane % GL, g = lane / GL;
+    const int T = static_cast<int>(p.T), chunks = D / 8, row_bytes = 2 * D, stage_bytes = ROWS * row_bytes;
+    uint4* hs = reinterpret_cast<uint4*>(ring + kFewWarps * stages * stage_bytes);  // [TT][D / 8]
+    const uint8_t* mine = ring + warp * stages * stage_bytes;
+    const uint32_t bar0 = smem_u32(bars + warp * kFewMaxStages);
     pdl_release();
+    if (lane < kFewMaxStages) mbar_init(bar0 + 8 * lane, 1);
+    fence_barrier_init();
+    __syncwarp();
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, T = static_cast<int>(p.T), chunks = D / 8;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.done = 0u;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * kFewWarps, per = (p.V + warps - 1) / warps;
+    const int v0 = static_cast<int>(min(static_cast<int64_t>(p.V), (static_cast<int64_t>(blockIdx.x) * kFewWarps + warp) * per));
+    const int n = static_cast<int>(min(static_cast<int64_t>(p.V) - v0, per));  // this warp's rows
+    auto fetch = [&](int i) {
+        const int rows = min(ROWS, n - i * ROWS);
+        if (rows <= 0) return;
+        const uint32_t bar = bar0 + 8 * (i % stages), dst = smem_u32(mine + (i % stages) * stage_bytes);
+        const uint16_t* src = weight + (static_cast<int64_t>(v0) + i * ROWS) * ldw;
+        mbar_arrive_expect_tx(bar, rows * row_bytes);
+        if (ldw == D) {
+            bulk_load(dst, src, rows * row_bytes, bar);
+        } else {
+            for (int r = 0; r < rows; ++r) bulk_load(dst + r * row_bytes, src + r * ldw, row_bytes, bar);
+        }
+    };
+    if (lane == 0)
+        for (int i = 0; i < stages; ++i) fetch(i);
     for (int i = threadIdx.x; i < TT * chunks; i += kFewThreads) {
         const int t = i / chunks;
         hs[i] = t < T ? *reinterpret_cast<const uint4*>(hidden + t * ldh + (i - t * chunks) * 8) : make_uint4(0, 0, 0, 0);
@@ -648,63 +679,57 @@ __global__ void __launch_bounds__(kFewThreads) vocab_few_kernel(const Rowwise p,
     float m[TT], s[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-        y[t] = t < T ? p.target[t] : -1;
+        y[t] = t < T ? p.target[t] - v0 : -1;
         m[t] = -INFINITY;
         s[t] = 0.f;
     }
-    const int warps = gridDim.x * (kFewThreads / 32);
-    const int per = (p.V + warps - 1) / warps;
-    const int v0 = min(static_cast<int64_t>(p.V), static_cast<int64_t>(blockIdx.x * (kFewThreads / 32) + warp) * per);
-    const int v1 = min(static_cast<int64_t>(p.V), static_cast<int64_t>(v0) + per);
-    for (int v = v0; v < v1; v += kFewRows) {
-        float acc[kFewRows][TT];
+    for (int i = 0; i * ROWS < n; ++i) {
+        if (!mbar_wait_warp(bar0 + 8 * (i % stages), (i / stages) & 1, status, K_VOCAB, 10)) {
+            for (int k = i + 1; k < i + stages && k * ROWS < n; ++k)  // the copies in flight
+                mbar_wait_warp(bar0 + 8 * (k % stages), (k / stages) & 1, status, K_VOCAB, 11);
+            break;
+        }
+        const uint4* row = reinterpret_cast<const uint4*>(mine + (i % stages) * stage_bytes + g * row_bytes);
+        float acc[TT][2];
 #pragma unroll
-        for (int r = 0; r < kFewRows; ++r)
+        for (int t = 0; t < TT; ++t) acc[t][0] = acc[t][1] = 0.f;
+#pragma unroll 4
+        for (int c = l; c < chunks; c += GL) {
+            float f[8];
+            unpack8<BF16>(row[c], f);
 #pragma unroll
-            for (int t = 0; t < TT; ++t) acc[r][t] = 0.f;
-        const uint16_t* w = weight + static_cast<int64_t>(v) * ldw;
-#pragma unroll 2
-        for (int c = lane; c < chunks; c += 32) {
-            uint4 x[kFewRows];
+            for (int t = 0; t < TT; ++t) {
+                float h[8];
+                unpack8<BF16>(hs[t * chunks + c], h);
 #pragma unroll
-            for (int r = 0; r < kFewRows; ++r)
-                x[r] = v + r < v1 ? __ldcs(reinterpret_cast<const uint4*>(w + r * ldw + c * 8)) : make_uint4(0, 0, 0, 0);
-            float h[TT][8];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) unpack8<BF16>(hs[t * chunks + c], h[t]);
-#pragma unroll
-            for (int r = 0; r < kFewRows; ++r) {
-                float f[8];
-                unpack8<BF16>(x[r], f);
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) acc[r][t] = fmaf(f[k], h[t][k], acc[r][t]);
+                for (int k = 0; k < 8; ++k) acc[t][k & 1] = fmaf(f[k], h[k], acc[t][k & 1]);
             }
         }
+        __syncwarp();
+        if (lane == 0) fetch(i + stages);
+        const int q = i * ROWS + g;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
+        for (int t = 0; t < TT; ++t) {
+            float z = acc[t][0] + acc[t][1];
 #pragma unroll
-            for (int r = 0; r < kFewRows; ++r)
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[r][t] += __shfl_xor_sync(0xffffffffu, acc[r][t], o);
-#pragma unroll
-        for (int r = 0; r < kFewRows; ++r)
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-                if (v + r < v1) {
-                    join(m[t], s[t], acc[r][t], acc[r][t] == acc[r][t] ? 1.f : acc[r][t]);
-                    if (lane == 0 && y[t] == v + r) p.zt[t] = acc[r][t];
-                }
+            for (int o = GL / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+            if (q < n) {
+                join(m[t], s[t], z, z == z ? 1.f : z);
+                if (l == 0 && y[t] == q) p.zt[t] = z;
+            }
+        }
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
+    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+        for (int o = GL; o < 32; o <<= 1) join(m[t], s[t], __shfl_xor_sync(0xffffffffu, m[t], o), __shfl_xor_sync(0xffffffffu, s[t], o));
         if (lane == 0) sh[warp][t] = make_float2(m[t], s[t]);
+    }
     __syncthreads();
     if (threadIdx.x < T) {
         const int t = threadIdx.x;
         float mm = -INFINITY, ss = 0.f;
-        for (int i = 0; i < kFewThreads / 32; ++i) join(mm, ss, sh[i][t].x, sh[i][t].y);
+        for (int i = 0; i < kFewWarps; ++i) join(mm, ss, sh[i][t].x, sh[i][t].y);
         p.part[static_cast<int64_t>(blockIdx.x) * T + t] = make_float2(mm, ss);
     }
 }
@@ -895,16 +920,14 @@ struct Bump {
     }
 };
 
-int64_t few_width(int64_t T) { return T <= 2 ? T : 4; }  // tokens that the kernel for T tokens is made for
+int few_width(int64_t T) { return T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8; }  // tokens that the kernel for T tokens is made for
 
 // Up to kFewTokens tokens skip the tensor cores; their pieces are the CTAs.
 bool few(const morpho_vocab_loss_t* p) {
-    return p->tokens <= kFewTokens && few_width(p->tokens) * p->dim * 2 <= 40 * 1024;  // the hidden rows' shared memory
+    return p->tokens <= kFewTokens && p->dim <= kFewMaxDim && few_width(p->tokens) * p->dim * 2 <= 32 * 1024;  // the hidden rows' shared memory
 }
 
-int few_blocks(const morpho_vocab_loss_t* p, int sms) {
-    return static_cast<int>(std::min<int64_t>(ceil_div(p->vocab, kFewRows * kFewThreads / 32), 3 * sms));
-}
+int few_blocks(const morpho_vocab_loss_t* p, int sms) { return static_cast<int>(std::min<int64_t>(ceil_div(p->vocab, kFewWarps), sms)); }
 
 int join_rows(int64_t T, int sms) {  // rows a block of the join takes: a power of two up to 32
     int r = 1;
@@ -1002,7 +1025,8 @@ int add_task(Launch* L, Task& t, int kind, bool a_mn, bool b_mn, int64_t M, int6
 template <bool BF16>
 int launch(const DeviceInfo& dev, Launch& L, cudaStream_t stream, const char* name) {
     auto kern = vocab_gemm_kernel<BF16>;
-    MORPHO_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    static SharedLimit limit;
+    MORPHO_CUDA_TRY(limit.raise(kern, dev.device, kSmemBytes));
     L.status = dev.status;
     const int pairs = std::min(L.task[L.tasks - 1].items_end, std::max(1, dev.sms / 2));
     prof_begin(stream, name);
@@ -1020,13 +1044,29 @@ int finish(const DeviceInfo& dev, const float* part, int slabs, int64_t elems, c
     return MORPHO_OK;
 }
 
-template <bool BF16, int TT>
-int launch_few(const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks, cudaStream_t stream) {
+template <bool BF16, int TT, int GL>
+int launch_few(const DeviceInfo& dev, const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks,
+               cudaStream_t stream) {
+    static SharedLimit limit;
+    const int stage = 32 / GL * 2 * p->dim;
+    const int stages = std::max(1, std::min(kFewMaxStages, kFewRing / (kFewWarps * stage)));
+    const int smem = kFewWarps * stages * stage + TT * 2 * p->dim;
+    auto kern = vocab_few_kernel<BF16, TT, GL>;
+    MORPHO_CUDA_TRY(limit.raise(kern, dev.device, smem));
     prof_begin(stream, "vocab_few");
-    MORPHO_CUDA_TRY(launch_after(vocab_few_kernel<BF16, TT>, blocks, kFewThreads, static_cast<size_t>(TT) * p->dim * 2, stream, r,
-                                 static_cast<const uint16_t*>(hidden), ld_hidden(p), static_cast<const uint16_t*>(weight), ld_weight(p), p->dim));
+    MORPHO_CUDA_TRY(launch_after(kern, blocks, kFewThreads, smem, stream, r, static_cast<const uint16_t*>(hidden), ld_hidden(p),
+                                 static_cast<const uint16_t*>(weight), ld_weight(p), p->dim, stages, dev.status));
     MORPHO_LAUNCH_CHECK("vocab_few");
     return MORPHO_OK;
+}
+
+// Lanes to a row: so many rows at a time that every warp has three stages of them in the ring.
+template <bool BF16, int TT>
+int launch_few(const DeviceInfo& dev, const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks,
+               cudaStream_t stream) {
+    return p->dim <= 1024   ? launch_few<BF16, TT, 8>(dev, r, p, hidden, weight, blocks, stream)
+           : p->dim <= 2048 ? launch_few<BF16, TT, 16>(dev, r, p, hidden, weight, blocks, stream)
+                            : launch_few<BF16, TT, 32>(dev, r, p, hidden, weight, blocks, stream);
 }
 
 int launch_join(const Rowwise& r, const FwdPlan& f, float* loss, float* lse, cudaStream_t stream) {
@@ -1061,9 +1101,11 @@ int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* h
     r.zt = f.zt;
     r.done = f.done;
     if (few(p)) {
-        MORPHO_TRY(p->tokens == 1   ? (launch_few<BF16, 1>(r, p, hidden, weight, f.pieces, stream))
-                   : p->tokens == 2 ? (launch_few<BF16, 2>(r, p, hidden, weight, f.pieces, stream))
-                                    : (launch_few<BF16, 4>(r, p, hidden, weight, f.pieces, stream)));
+        const int w = few_width(p->tokens);
+        MORPHO_TRY(w == 1   ? (launch_few<BF16, 1>(dev, r, p, hidden, weight, f.pieces, stream))
+                   : w == 2 ? (launch_few<BF16, 2>(dev, r, p, hidden, weight, f.pieces, stream))
+                   : w == 4 ? (launch_few<BF16, 4>(dev, r, p, hidden, weight, f.pieces, stream))
+                            : (launch_few<BF16, 8>(dev, r, p, hidden, weight, f.pieces, stream)));
     } else {
         Launch L{};
         L.rows = r;
