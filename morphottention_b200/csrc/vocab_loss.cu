@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(256) vocab_finish_kernel(const float* part, in
 
 // ---- a few tokens: logits on CUDA cores ------------------------------------------------------------
 
-constexpr int kFewTokens = 8;
+constexpr int kFewTokens = 2;  // (32768 x 1024: 16 and 19 us; with three or four 26, and the tensor cores take 25 for any number up to 256)
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kFewMaxStages = 6, kFewRing = 192 * 1024;
@@ -631,14 +631,14 @@ __device__ __forceinline__ void unpack8(uint4 x, float* f) {
 }
 
 // Up to TT tokens against the whole vocabulary, bound by reading the weight once.  Each warp streams a
-// contiguous range of rows through a ring of its own in shared memory (bulk copies of 32 / GL rows), so the
-// bytes in flight do not hang on registers; GL lanes share a row, the groups of a warp work on as many rows,
-// each keeping the running maximum and sum of its own.  The hidden rows stand in shared memory too, and every
+// contiguous range of rows through a ring of its own in shared memory (bulk copies of R 32 / GL rows), so the
+// bytes in flight do not hang on registers; GL lanes share R rows, the groups of a warp work on as many, each
+// keeping the running maximum and sum of its own.  The hidden rows stand in shared memory too, and every
 // CTA (one per SM) leaves one piece of each token's statistics.
-template <bool BF16, int TT, int GL>
+template <bool BF16, int TT, int GL, int R>
 __global__ void __launch_bounds__(kFewThreads, 1) vocab_few_kernel(const Rowwise p, const uint16_t* hidden, int64_t ldh, const uint16_t* weight,
                                                                    int64_t ldw, int D, int stages, uint32_t* status) {
-    constexpr int ROWS = 32 / GL;  // at a time
+    constexpr int GROUPS = 32 / GL, ROWS = R * GROUPS;  // rows at a time: g, g + GROUPS of every stage
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ uint64_t bars[kFewWarps * kFewMaxStages];
     __shared__ float2 sh[kFewWarps][TT];
@@ -690,32 +690,40 @@ __global__ void __launch_bounds__(kFewThreads, 1) vocab_few_kernel(const Rowwise
             break;
         }
         const uint4* row = reinterpret_cast<const uint4*>(mine + (i % stages) * stage_bytes + g * row_bytes);
-        float acc[TT][2];
+        float acc[R][TT][2];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) acc[t][0] = acc[t][1] = 0.f;
-#pragma unroll 4
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[r][t][0] = acc[r][t][1] = 0.f;
+#pragma unroll 2
         for (int c = l; c < chunks; c += GL) {
-            float f[8];
-            unpack8<BF16>(row[c], f);
+            float f[R][8];
+#pragma unroll
+            for (int r = 0; r < R; ++r) unpack8<BF16>(row[r * GROUPS * chunks + c], f[r]);
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
                 float h[8];
                 unpack8<BF16>(hs[t * chunks + c], h);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) acc[t][k & 1] = fmaf(f[k], h[k], acc[t][k & 1]);
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) acc[r][t][k & 1] = fmaf(f[r][k], h[k], acc[r][t][k & 1]);
             }
         }
         __syncwarp();
         if (lane == 0) fetch(i + stages);
-        const int q = i * ROWS + g;
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            float z = acc[t][0] + acc[t][1];
+        for (int r = 0; r < R; ++r) {
+            const int q = i * ROWS + r * GROUPS + g;
 #pragma unroll
-            for (int o = GL / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-            if (q < n) {
-                join(m[t], s[t], z, z == z ? 1.f : z);
-                if (l == 0 && y[t] == q) p.zt[t] = z;
+            for (int t = 0; t < TT; ++t) {
+                float z = acc[r][t][0] + acc[r][t][1];
+#pragma unroll
+                for (int o = GL / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+                if (q < n) {  // (a short last stage holds older rows past it)
+                    join(m[t], s[t], z, z == z ? 1.f : z);
+                    if (l == 0 && y[t] == q) p.zt[t] = z;
+                }
             }
         }
     }
@@ -852,15 +860,17 @@ __global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, floa
 constexpr size_t kPieceBytes = 512u << 20;  // dz of one piece of the vocabulary, at most; two are held
 // Terms of one tensor-core sum, at most.  The tensor core truncates its fp32 accumulator at every
 // K = 16 step, which biases a long sum towards zero (2.3e-8 of it a step; 1.2 % measured after 2^23
-// terms), so longer sums are joined from sums of this length by rounded fp32 additions.
-constexpr int kMaxK = 16384;
+// terms), so longer sums are joined from sums of this length (5e-5, a fifth of fp16's own rounding) by
+// rounded fp32 additions.
+constexpr int kMaxK = 32768;
+constexpr int kMaxDim = 16384;
 
 int validate_loss(const morpho_vocab_loss_t* p) {
     if (p == nullptr) return set_error(MORPHO_ERR_INVALID, "cross entropy problem is NULL");
     if (p->tokens < 0 || p->tokens > (1LL << 30)) return set_error(MORPHO_ERR_INVALID, "cross entropy: tokens = %lld out of range", static_cast<long long>(p->tokens));
     if (p->vocab <= 0 || p->vocab > (1 << 30)) return set_error(MORPHO_ERR_INVALID, "cross entropy: vocab = %d out of range", p->vocab);
-    if (p->dim <= 0 || p->dim > kMaxK || p->dim % 8 != 0)
-        return set_error(MORPHO_ERR_INVALID, "cross entropy: dim = %d must be a positive multiple of 8, at most %d", p->dim, kMaxK);
+    if (p->dim <= 0 || p->dim > kMaxDim || p->dim % 8 != 0)
+        return set_error(MORPHO_ERR_INVALID, "cross entropy: dim = %d must be a positive multiple of 8, at most %d", p->dim, kMaxDim);
     if (p->type != MORPHO_DTYPE_F16 && p->type != MORPHO_DTYPE_BF16)
         return set_error(MORPHO_ERR_INVALID, "cross entropy: hidden and weight must be fp16 or bf16");
     if (p->reduction < MORPHO_REDUCTION_NONE || p->reduction > MORPHO_REDUCTION_SUM)
@@ -920,11 +930,9 @@ struct Bump {
     }
 };
 
-int few_width(int64_t T) { return T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8; }  // tokens that the kernel for T tokens is made for
-
 // Up to kFewTokens tokens skip the tensor cores; their pieces are the CTAs.
 bool few(const morpho_vocab_loss_t* p) {
-    return p->tokens <= kFewTokens && p->dim <= kFewMaxDim && few_width(p->tokens) * p->dim * 2 <= 32 * 1024;  // the hidden rows' shared memory
+    return p->tokens <= kFewTokens && p->dim <= kFewMaxDim;
 }
 
 int few_blocks(const morpho_vocab_loss_t* p, int sms) { return static_cast<int>(std::min<int64_t>(ceil_div(p->vocab, kFewWarps), sms)); }
@@ -1044,14 +1052,14 @@ int finish(const DeviceInfo& dev, const float* part, int slabs, int64_t elems, c
     return MORPHO_OK;
 }
 
-template <bool BF16, int TT, int GL>
+template <bool BF16, int TT, int GL, int R>
 int launch_few(const DeviceInfo& dev, const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks,
                cudaStream_t stream) {
     static SharedLimit limit;
-    const int stage = 32 / GL * 2 * p->dim;
+    const int stage = R * 32 / GL * 2 * p->dim;
     const int stages = std::max(1, std::min(kFewMaxStages, kFewRing / (kFewWarps * stage)));
     const int smem = kFewWarps * stages * stage + TT * 2 * p->dim;
-    auto kern = vocab_few_kernel<BF16, TT, GL>;
+    auto kern = vocab_few_kernel<BF16, TT, GL, R>;
     MORPHO_CUDA_TRY(limit.raise(kern, dev.device, smem));
     prof_begin(stream, "vocab_few");
     MORPHO_CUDA_TRY(launch_after(kern, blocks, kFewThreads, smem, stream, r, static_cast<const uint16_t*>(hidden), ld_hidden(p),
@@ -1064,9 +1072,10 @@ int launch_few(const DeviceInfo& dev, const Rowwise& r, const morpho_vocab_loss_
 template <bool BF16, int TT>
 int launch_few(const DeviceInfo& dev, const Rowwise& r, const morpho_vocab_loss_t* p, const void* hidden, const void* weight, int blocks,
                cudaStream_t stream) {
-    return p->dim <= 1024   ? launch_few<BF16, TT, 8>(dev, r, p, hidden, weight, blocks, stream)
-           : p->dim <= 2048 ? launch_few<BF16, TT, 16>(dev, r, p, hidden, weight, blocks, stream)
-                            : launch_few<BF16, TT, 32>(dev, r, p, hidden, weight, blocks, stream);
+    return p->dim <= 512    ? launch_few<BF16, TT, 8, 2>(dev, r, p, hidden, weight, blocks, stream)
+           : p->dim <= 1024 ? launch_few<BF16, TT, 8, 1>(dev, r, p, hidden, weight, blocks, stream)
+           : p->dim <= 2048 ? launch_few<BF16, TT, 16, 1>(dev, r, p, hidden, weight, blocks, stream)
+                            : launch_few<BF16, TT, 32, 1>(dev, r, p, hidden, weight, blocks, stream);
 }
 
 int launch_join(const Rowwise& r, const FwdPlan& f, float* loss, float* lse, cudaStream_t stream) {
@@ -1101,11 +1110,8 @@ int forward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const void* h
     r.zt = f.zt;
     r.done = f.done;
     if (few(p)) {
-        const int w = few_width(p->tokens);
-        MORPHO_TRY(w == 1   ? (launch_few<BF16, 1>(dev, r, p, hidden, weight, f.pieces, stream))
-                   : w == 2 ? (launch_few<BF16, 2>(dev, r, p, hidden, weight, f.pieces, stream))
-                   : w == 4 ? (launch_few<BF16, 4>(dev, r, p, hidden, weight, f.pieces, stream))
-                            : (launch_few<BF16, 8>(dev, r, p, hidden, weight, f.pieces, stream)));
+        MORPHO_TRY(p->tokens == 1 ? (launch_few<BF16, 1>(dev, r, p, hidden, weight, f.pieces, stream))
+                                  : (launch_few<BF16, 2>(dev, r, p, hidden, weight, f.pieces, stream)));
     } else {
         Launch L{};
         L.rows = r;
