@@ -18,8 +18,8 @@
 //
 // The GEMMs run as 256 x 256 tiles of CTA pairs (cta_group::2): each SM reads half of A's rows and half of
 // B's columns, 32 KB for every 64 of K, where a 128 x 256 tile of one CTA reads 48 KB and leaves its
-// shared memory port busier than its tensor core.  Warp roles (352 threads): warp 0 TMA producer, warp 1
-// MMA issuer (rank 0 of the pair), warps 2-9 epilogue, warp 10 scheduler; the accumulator is double-buffered in TMEM, and
+// shared memory port busier than its tensor core.  Warp roles (608 threads): warp 0 TMA producer, warp 1
+// MMA issuer (rank 0 of the pair), warps 2-17 epilogue, warp 18 scheduler; the accumulator is double-buffered in TMEM, and
 // results leave through TMA stores from a swizzled box per warp.
 #include <algorithm>
 #include <type_traits>
@@ -35,13 +35,19 @@ constexpr uint32_t K_VOCAB = 6;  // kernel id in the device status word
 constexpr int kTile = 256;       // rows and columns of a CTA pair's tile
 constexpr int kHalf = 128;       // rows of A, columns of B, and rows of the tile that one CTA holds
 constexpr int BK = 128;          // K of a stage
-constexpr int kGemmThreads = 352;
+constexpr int kEpiWarps = 16;    // two sets of eight, which take the tiles in turn: while one set's loads and
+                                 // stores wait, the other's exponentials run
+constexpr int kSetWarps = 8;
+constexpr int kPiece = 128;      // columns of a tile that one warp takes,
+constexpr int kLoad = 64;        // so many at once
+constexpr int kGemmThreads = 32 * (kEpiWarps + 3);
 constexpr int kStages = 3;
 constexpr int kPanel = kHalf * 128;         // 16 KB: 128 rows of 128 bytes
 constexpr int kOperandBytes = 2 * kPanel;   // 128 x 128 elements: two panels side by side
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kStoreOffset = kStages * kStageBytes;  // a 4 KB box for each epilogue warp's stores
-constexpr int kBarOffset = kStoreOffset + 8 * 4096;
+constexpr int kBoxBytes = 2048;                      // of an epilogue warp's stores: 32 rows of 64 bytes
+constexpr int kStoreOffset = kStages * kStageBytes;  // a box for each of them
+constexpr int kBarOffset = kStoreOffset + kEpiWarps * kBoxBytes;
 constexpr int kSmemBytes = kBarOffset + 512 + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory");
 
@@ -54,6 +60,20 @@ enum Kind : int {
     kPartAdd // the same, added to what is there
 };
 
+// n / d for 0 <= n < 2^31 by one multiplication: mul = ceil(2^(32 + shift) / d), 2^shift the power of two not below d.
+struct FastDiv {
+    uint32_t mul, shift, d;
+    static FastDiv of(int d) {
+        FastDiv f{0, 0, static_cast<uint32_t>(d)};
+        while ((1u << f.shift) < f.d) ++f.shift;
+        f.mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << f.shift) - f.d)) / f.d + 1);
+        return f;
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return static_cast<int>((__umulhi(mul, static_cast<uint32_t>(n)) + static_cast<uint32_t>(n)) >> shift);
+    }
+};
+
 // D (M x N) = A (M x K) B (K x N) as 256 x 256 tiles of CTA pairs, K cut into splits.
 struct alignas(64) Task {
     CUtensorMap a, b, out;
@@ -63,9 +83,10 @@ struct alignas(64) Task {
     int a_row0, b_row0;  // first row of A / B in its map
     int M, N;
     int tiles_m, tiles_n, group;  // `group` M tiles share each B tile in L2
+    FastDiv by_slab, by_band, by_group, by_last;  // tiles; group x N tiles; group; M tiles of the last group
     int K, k_blocks, kb_per_split;
     int items_end;  // work items of this task and those before it
-    int v0;         // kDz: the piece's first column of the vocabulary
+    int v0, padded; // kDz: the piece's first column of the vocabulary; its width in whole panels
 };
 
 // What the epilogues and the row kernels know of the rows.  A target that is neither in [0, V) nor
@@ -76,13 +97,13 @@ struct Rowwise {
     const int64_t* target;
     int64_t ignore_index;
     int reduction;
-    float2* part;   // forward: [pieces][T] maximum and sum of each piece of a row
+    float2* part;   // forward: [pieces][T] maximum and sum of each piece of a row (kPiece columns, or a CTA's)
     float* zt;      // forward: [T] logit of the target
     uint32_t* done; // forward: the join kernel's count of finished blocks
     const float* lse;
     const float* grad;
     const float* row_scale;  // r_t unit (0 for ignored rows); NULL: unit, or 0
-    float unit;
+    float unit, log2_unit;
     float* common;  // gmax / unit, the factor of the results
 };
 
@@ -106,72 +127,82 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return pack_half2(lo, hi);
 }
 
-// ---- epilogues: one thread per row, 128 columns at `tacc` ------------------------------------------
+// ---- epilogues: one thread per row, kPiece columns at `tacc` ---------------------------------------
 
-// Writes one 4 KB box (32 rows of 128 bytes, this lane's row in `x`) to this warp's staging buffer in the
-// TMA's 128-byte swizzle; lane 0 may then store it.
+// Writes one box (32 rows of 64 bytes, this lane's row in `x`) to this warp's staging buffer in the TMA's
+// 64-byte swizzle; lane 0 may then store it.
 __device__ __forceinline__ void stage_box(uint32_t stage, int lane, const uint32_t* x) {
     if (lane == 0) bulk_wait_read_all();  // the previous box has left
     __syncwarp();
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
-        st_shared_u4(stage + lane * 128 + ((g ^ (lane & 7)) << 4), make_uint4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]));
+    for (int g = 0; g < 4; ++g)
+        st_shared_u4(stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4), make_uint4(x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]));
     fence_proxy_async_smem();
     __syncwarp();
 }
 
-// The warp's 128 columns of its 32 rows, after which the accumulator may be written again.
-template <class Release>
-__device__ __forceinline__ void load_piece(uint32_t tacc, uint32_t* r, Release release) {
+// f(registers, column) for the warp's columns of its 32 rows, kLoad at a time; `release` after the last load,
+// when the accumulator may be written again.
+template <class Release, class F>
+__device__ __forceinline__ void each_load(uint32_t tacc, Release release, F f) {
+#pragma unroll 1
+    for (int c = 0; c < kPiece; c += kLoad) {
+        uint32_t r[kLoad];
+        __syncwarp();
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 32) tmem_ld32(tacc + c, r + c);
-    tmem_ld_wait();
-    release();
+        for (int i = 0; i < kLoad; i += 32) tmem_ld32(tacc + c + i, r + i);
+        tmem_ld_wait();
+        if (c + kLoad == kPiece) release();
+        f(r, c);
+    }
 }
 
 // Row statistics: the piece's maximum and sum of exp(z - maximum), and the target's logit.  Four
-// independent chains each for the maximum and the sum: two warps per scheduler hide little latency.
+// independent chains each for the maximum and the sum.
 template <class Release>
 __device__ __forceinline__ void epi_stats(const Rowwise& p, uint32_t tacc, int64_t row, int n0, Release release) {
     const int64_t y = (row < p.T ? p.target[row] : -1) - n0;
-    uint32_t r[kHalf];
-    load_piece(tacc, r, release);
-    if (n0 + kHalf > p.V) {  // columns past the vocabulary
+    float m = -INFINITY, s = 0.f, zt = 0.f;
+    each_load(tacc, release, [&](uint32_t* r, int c) {
+        const int left = p.V - n0 - c;
+        if (left < kLoad) {  // columns past the vocabulary
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-            if (i >= p.V - n0) r[i] = __float_as_uint(-INFINITY);
-    }
-    float m4[4], s4[4];
+            for (int i = 0; i < kLoad; ++i)
+                if (i >= left) r[i] = __float_as_uint(-INFINITY);
+        }
+        float m4[4], s4[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        m4[c] = u2f(r[c]);
-        s4[c] = 0.f;
-    }
+        for (int k = 0; k < 4; ++k) {
+            m4[k] = u2f(r[k]);
+            s4[k] = 0.f;
+        }
 #pragma unroll
-    for (int i = 4; i + 8 <= kHalf; i += 8)
+        for (int i = 4; i + 8 <= kLoad; i += 8)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) m4[c] = fmax3(m4[c], u2f(r[i + c]), u2f(r[i + 4 + c]));
+            for (int k = 0; k < 4; ++k) m4[k] = fmax3(m4[k], u2f(r[i + k]), u2f(r[i + 4 + k]));
 #pragma unroll
-    for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], u2f(r[kHalf - 4 + c]));
-    const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-    float zt = 0.f;
-    if (__any_sync(0xffffffffu, y >= 0 && y < kHalf)) {
+        for (int k = 0; k < 4; ++k) m4[k] = fmaxf(m4[k], u2f(r[kLoad - 4 + k]));
+        const float mn = fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+        if (__any_sync(0xffffffffu, y >= c && y < c + kLoad)) {
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-            if (i == y) zt = u2f(r[i]);
-    }
-    const float b = m > -INFINITY ? m * kLog2e : 0.f;  // -inf throughout, or NaN (which a maximum skips)
+            for (int i = 0; i < kLoad; ++i)
+                if (c + i == y) zt = u2f(r[i]);
+        }
+        const float b = mn > -INFINITY ? mn * kLog2e : 0.f;  // -inf throughout, or NaN (which a maximum skips)
 #pragma unroll
-    for (int i = 0; i < kHalf; i += 4)
+        for (int i = 0; i < kLoad; i += 4)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s4[c] += ex2(fmaf(u2f(r[i + c]), kLog2e, -b));
+            for (int k = 0; k < 4; ++k) s4[k] += ex2(fmaf(u2f(r[i + k]), kLog2e, -b));
+        s = s * ex2(fmaf(m, kLog2e, -b)) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+        m = mn;
+    });
     if (row < p.T) {
-        p.part[static_cast<int64_t>(n0 / kHalf) * p.T + row] = make_float2(m, (s4[0] + s4[1]) + (s4[2] + s4[3]));
-        if (y >= 0 && y < kHalf && y + n0 < p.V) p.zt[row] = zt;
+        p.part[static_cast<int64_t>(n0 / kPiece) * p.T + row] = make_float2(m, s);
+        if (y >= 0 && y < kPiece && y + n0 < p.V) p.zt[row] = zt;
     }
 }
 
-// dz of one piece: r_t (exp(z - lse) - [v = target]).
+// dz of one piece: r_t (exp(z - lse) - [v = target]), r_t in the exponent where it is the same for all rows.
 template <bool BF16, class Release>
 __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t tacc, int64_t row, int row0, int n0,
                                        uint32_t stage, int lane, Release release) {
@@ -179,40 +210,46 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
     const int64_t target = live ? p.target[row] : -1;
     const int64_t y = target - t.v0 - n0;
     const float l2 = live ? p.lse[row] * kLog2e : 0.f;
-    const float rs = !live                    ? 0.f
-                     : p.row_scale != nullptr ? p.row_scale[row]
-                                              : (target != p.ignore_index ? p.unit : 0.f);
-    uint32_t r[kHalf];
-    load_piece(tacc, r, release);
-    const bool hit = __any_sync(0xffffffffu, y >= 0 && y < kHalf);
+    const bool own = p.row_scale != nullptr;
+    const float rs = !live ? 0.f : own ? p.row_scale[row] : (target != p.ignore_index ? p.unit : 0.f);
+    const float shift = own ? -l2 : p.log2_unit - l2;
+    each_load(tacc, release, [&](uint32_t* r, int c) {
+        const bool hit = __any_sync(0xffffffffu, y >= c && y < c + kLoad);
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        if (n0 + b * 64 < t.N) {
-            uint32_t x[32];
+        for (int b = 0; b < kLoad; b += 32) {
+            const int col = n0 + c + b;
+            if (col < t.padded) {
+                uint32_t* q = r + b;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) r[b * 64 + i] = __float_as_uint(rs * ex2(fmaf(u2f(r[b * 64 + i]), kLog2e, -l2)));
-            if (n0 + b * 64 + 64 > t.N) {  // the last panel's columns past the piece are read as K: zeros
+                for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(ex2(fmaf(u2f(q[i]), kLog2e, shift)));
+                if (own) {
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (n0 + b * 64 + i >= t.N) r[b * 64 + i] = 0u;
-            }
-            if (hit) {
+                    for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(rs * u2f(q[i]));
+                }
+                if (col + 32 > t.N) {  // columns past the piece, which are read as K: zeros
 #pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (b * 64 + i == y) r[b * 64 + i] = __float_as_uint(u2f(r[b * 64 + i]) - rs);
-            }
+                    for (int i = 0; i < 32; ++i)
+                        if (col + i >= t.N) q[i] = 0u;
+                }
+                if (hit) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                x[i] = pack2<BF16>(u2f(r[b * 64 + 2 * i]), u2f(r[b * 64 + 2 * i + 1]));
-                if (rs == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
-            }
-            stage_box(stage, lane, x);
-            if (lane == 0 && row0 < t.M) {
-                tma_store_2d(&t.out, stage, n0 + b * 64, row0);
-                bulk_commit_group();
+                    for (int i = 0; i < 32; ++i)
+                        if (c + b + i == y) q[i] = __float_as_uint(u2f(q[i]) - rs);
+                }
+                uint32_t x[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = pack2<BF16>(u2f(q[2 * i]), u2f(q[2 * i + 1]));
+                    if (rs == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
+                }
+                stage_box(stage, lane, x);
+                if (lane == 0 && row0 < t.M) {
+                    tma_store_2d(&t.out, stage, col, row0);
+                    bulk_commit_group();
+                }
             }
         }
-    }
+    });
 }
 
 // 16-bit result: common * sum.
@@ -220,48 +257,42 @@ template <bool BF16, class Release>
 __device__ __forceinline__ void epi_out(const Rowwise& p, const Task& t, uint32_t tacc, int row0, int n0, uint32_t stage,
                                         int lane, Release release) {
     const float g = *p.common;
-    const int boxes = min(2, (t.N - n0 + 63) / 64);
-#pragma unroll 1
-    for (int b = 0; b < boxes; ++b) {
-        uint32_t x[32];
+    each_load(tacc, release, [&](uint32_t* r, int c) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            uint32_t r[32];
-            __syncwarp();
-            tmem_ld32(tacc + b * 64 + q * 32, r);
-            tmem_ld_wait();
-            if (q == 1 && b == boxes - 1) release();
+        for (int b = 0; b < kLoad; b += 32) {
+            if (n0 + c + b < t.N) {
+                uint32_t x[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[q * 16 + i] = pack2<BF16>(g * u2f(r[2 * i]), g * u2f(r[2 * i + 1]));
+                for (int i = 0; i < 16; ++i) x[i] = pack2<BF16>(g * u2f(r[b + 2 * i]), g * u2f(r[b + 2 * i + 1]));
+                stage_box(stage, lane, x);
+                if (lane == 0 && row0 < t.M) {
+                    tma_store_2d(&t.out, stage, n0 + c + b, row0);
+                    bulk_commit_group();
+                }
+            }
         }
-        stage_box(stage, lane, x);
-        if (lane == 0 && row0 < t.M) {
-            tma_store_2d(&t.out, stage, n0 + b * 64, row0);
-            bulk_commit_group();
-        }
-    }
+    });
 }
 
 // fp32 partial sums of K split z.
 template <class Release>
 __device__ __forceinline__ void epi_part(const Task& t, uint32_t tacc, int row0, int n0, int z, uint32_t stage, int lane,
                                          Release release) {
-    const int boxes = min(4, (t.N - n0 + 31) / 32);
-#pragma unroll 1
-    for (int b = 0; b < boxes; ++b) {
-        uint32_t r[32];
-        tmem_ld32(tacc + b * 32, r);
-        tmem_ld_wait();
-        if (b == boxes - 1) release();
-        stage_box(stage, lane, r);
-        if (lane == 0 && row0 < t.M) {
-            if (t.kind == kPartAdd)
-                tma_reduce_add_3d(&t.out, stage, n0 + b * 32, row0, z);
-            else
-                tma_store_3d(&t.out, stage, n0 + b * 32, row0, z);
-            bulk_commit_group();
+    each_load(tacc, release, [&](uint32_t* r, int c) {
+#pragma unroll
+        for (int b = 0; b < kLoad; b += 16) {
+            if (n0 + c + b < t.N) {
+                stage_box(stage, lane, r + b);
+                if (lane == 0 && row0 < t.M) {
+                    if (t.kind == kPartAdd)
+                        tma_reduce_add_3d(&t.out, stage, n0 + c + b, row0, z);
+                    else
+                        tma_store_3d(&t.out, stage, n0 + c + b, row0, z);
+                    bulk_commit_group();
+                }
+            }
         }
-    }
+    });
 }
 
 // ---- the GEMM: up to three tasks in one persistent launch of CTA pairs -----------------------------
@@ -279,14 +310,13 @@ __device__ __forceinline__ Item item_of(const Launch& L, int w) {
     while (w >= L.task[i].items_end) start = L.task[i++].items_end;
     const Task& t = L.task[i];
     int r = w - start;
-    const int mn = t.tiles_m * t.tiles_n;
     it.task = i;
-    it.z = r / mn;
-    r -= it.z * mn;
-    const int g = r / (t.group * t.tiles_n);
-    r -= g * t.group * t.tiles_n;
-    const int gm = min(t.group, t.tiles_m - g * t.group);
-    const int n = r / gm;
+    it.z = t.by_slab.div(r);
+    r -= it.z * static_cast<int>(t.by_slab.d);
+    const int g = t.by_band.div(r);
+    r -= g * static_cast<int>(t.by_band.d);
+    const FastDiv& by = (g + 1) * t.group <= t.tiles_m ? t.by_group : t.by_last;
+    const int n = by.div(r), gm = static_cast<int>(by.d);
     it.m0 = (g * t.group + r - n * gm) * kTile;
     it.n0 = n * kTile;
     return it;
@@ -381,7 +411,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     if (threadIdx.x == 0) {
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(items.full0 + 8 * s, 1);    // rank 0's scheduler, to both
-            mbar_init(items.empty0 + 8 * s, 19);  // used in rank 0: its MMA thread, 2 producers, 16 epilogue warps
+            mbar_init(items.empty0 + 8 * s, 3 + 2 * kSetWarps);  // used in rank 0: its MMA thread, both CTAs' producers and one set
         }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, 1);   // used in rank 0: its producer's arrival and both CTAs' bytes
@@ -389,7 +419,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_full0 + 8 * a, 1);    // rank 0's commit, to both
-            mbar_init(acc_empty0 + 8 * a, 16);  // used in rank 0: the epilogue warps of both
+            mbar_init(acc_empty0 + 8 * a, 2 * kSetWarps);  // used in rank 0: the buffer's epilogue set of both
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
@@ -511,25 +541,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
             }
             if (lane == 0) *L.rows.common = *L.rows.grad / (static_cast<float>(max(kept, int64_t(1))) * L.rows.unit);
         }
-    } else if (warp == 10) {
+    } else if (warp == kEpiWarps + 2) {
         // ---------------- scheduler, one thread of rank 0 ----------------
         if (rank == 0 && lane == 0 && L.next != nullptr) {
             Item it = item_of(L, first);
-            for (int j = 1; it.task >= 0; ++j) {
+            // the end is published twice: each epilogue set reads every other item
+            for (int j = 1, ends = it.task < 0; ends < 2; ++j) {
                 if (!items.room(j, L.status)) {
                     *abort_flag = 1u;
                     break;
                 }
-                it = item_of(L, step + static_cast<int>(atomicAdd(L.next, 1u)));
+                if (ends == 0) it = item_of(L, step + static_cast<int>(atomicAdd(L.next, 1u)));
+                ends += it.task < 0;
                 items.publish(j, it);
             }
         }
     } else {
         // ---------------- epilogue, in both CTAs ----------------
-        const int quad = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t stage = smem_u32(smem + kStoreOffset + (warp - 2) * 4096);
+        const int set = (warp - 2) / kSetWarps, quad = warp & 3, piece = ((warp - 2) >> 2) & 1;
+        const uint32_t stage = smem_u32(smem + kStoreOffset + (warp - 2) * kBoxBytes);
         Item it = item_of(L, first);
-        for (int j = 0;; ++j) {
+        for (int j = set;; j += 2) {  // set 0 the even items, set 1 the odd ones
             if (j > 0) {
                 const bool ok = items.read(j, it, L, first, step);
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -546,14 +578,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                 break;
             }
             tc_fence_after();
-            const int row0 = it.m0 + rank * kHalf + quad * 32, n0 = it.n0 + half * kHalf;
-            const uint32_t tacc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + a * kTile + half * kHalf;
+            const int row0 = it.m0 + rank * kHalf + quad * 32, n0 = it.n0 + piece * kPiece;
+            const uint32_t tacc = tmem + (static_cast<uint32_t>(quad * 32) << 16) + a * kTile + piece * kPiece;
             auto release = [&]() {  // this warp has read its part of the accumulator
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * a, 0));
             };
-            if (n0 >= t.N) {
+            if (n0 >= t.N) {  // (dz: its padding ends inside the last live piece)
                 release();
             } else if (t.kind == kStats) {
                 epi_stats(L.rows, tacc, static_cast<int64_t>(row0) + lane, n0, release);
@@ -952,7 +984,7 @@ struct FwdPlan {
 };
 void plan_forward(Bump& b, const morpho_vocab_loss_t* p, int sms, FwdPlan* f) {
     const size_t T = p->tokens;
-    f->pieces = few(p) ? few_blocks(p, sms) : static_cast<int>(ceil_div(p->vocab, kHalf));
+    f->pieces = few(p) ? few_blocks(p, sms) : static_cast<int>(ceil_div(p->vocab, kPiece));
     f->rows = join_rows(T, sms);
     f->part = b.take<float2>(f->pieces * T);
     f->zt = b.take<float>(T);
@@ -997,15 +1029,15 @@ int load_map(CUtensorMap* m, bool* whole, const void* base, int64_t rows, int64_
     const uint32_t box[3] = {64, 128, 2};
     return make_tmap(m, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// Stores of 32 rows x 128 bytes: a 16-bit matrix, and fp32 slabs [slabs, rows, cols].
+// Stores of 32 rows x 64 bytes: a 16-bit matrix, and fp32 slabs [slabs, rows, cols].
 int store_map(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t ld) {
-    return make_tmap_2d_f16(m, base, rows, cols, ld, 32, 64);
+    return make_tmap_2d_f16(m, base, rows, cols, ld, 32, 32);
 }
 int slab_map(CUtensorMap* m, const void* base, int64_t slabs, int64_t rows, int64_t cols) {
     const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), static_cast<uint64_t>(slabs)};
     const uint64_t strides[2] = {static_cast<uint64_t>(cols) * 4, static_cast<uint64_t>(rows) * cols * 4};
-    const uint32_t box[3] = {32, 32, 1};
-    return make_tmap(m, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t box[3] = {16, 32, 1};
+    return make_tmap(m, base, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Appends a task whose maps are set.
@@ -1019,6 +1051,10 @@ int add_task(Launch* L, Task& t, int kind, bool a_mn, bool b_mn, int64_t M, int6
     t.tiles_n = static_cast<int>(ceil_div(N, kTile));
     // 16 M tiles x about 5 N tiles at a time on 74 CTA pairs (8 x 9: 2 % slower); a few N tiles run side by side
     t.group = t.tiles_n <= 8 ? 1 : 16;
+    t.by_slab = FastDiv::of(t.tiles_m * t.tiles_n);
+    t.by_band = FastDiv::of(t.group * t.tiles_n);
+    t.by_group = FastDiv::of(t.group);
+    t.by_last = FastDiv::of(t.tiles_m % t.group == 0 ? t.group : t.tiles_m % t.group);
     t.K = static_cast<int>(K);
     t.k_blocks = static_cast<int>(ceil_div(K, BK));
     t.kb_per_split = static_cast<int>(ceil_div(t.k_blocks, splits));
@@ -1133,6 +1169,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
     r.lse = lse;
     r.grad = grad;
     r.unit = BF16 ? 1.0f : 32768.0f;
+    r.log2_unit = BF16 ? 0.0f : 15.0f;
     r.common = f.common;
     if (p->reduction == MORPHO_REDUCTION_NONE) {
         prof_begin(stream, "vocab_scale");
@@ -1183,9 +1220,10 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
             Task z{};
             z.v0 = (i + 1) * c.cols;
             z.b_row0 = z.v0;
+            z.padded = static_cast<int>(ceil_div(width(i + 1), 64) * 64);
             MORPHO_TRY(load_map(&z.a, &z.a_whole, hidden, T, D, ld_hidden(p)));
             MORPHO_TRY(load_map(&z.b, &z.b_whole, weight, p->vocab, D, ld_weight(p)));
-            MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, ceil_div(width(i + 1), 64) * 64, c.cols));
+            MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, z.padded, c.cols));
             MORPHO_TRY(add_task(&L, z, kDz, false, false, T, width(i + 1), D, 1));
         }
         MORPHO_TRY(launch<BF16>(dev, L, stream, i < 0 ? "vocab_dz" : "vocab_grad"));
