@@ -97,12 +97,13 @@ struct Rowwise {
     const int64_t* target;
     int64_t ignore_index;
     int reduction;
+    float unbias, log2e;  // what makes up for the tensor core's truncation of a logit (unbias_of), and log2(e) times it
     float2* part;   // forward: [pieces][T] maximum and sum of each piece of a row (kPiece columns, or a CTA's)
     float* zt;      // forward: [T] logit of the target
     uint32_t* done; // forward: the join kernel's count of finished blocks
     const float* lse;
     const float* grad;
-    const float* row_scale;  // r_t unit (0 for ignored rows); NULL: unit, or 0
+    const float* row_scale;  // r_t (0 for ignored rows); NULL: 1, or 0
     float unit, log2_unit;
     float* common;  // gmax / unit, the factor of the results
 };
@@ -188,21 +189,21 @@ __device__ __forceinline__ void epi_stats(const Rowwise& p, uint32_t tacc, int64
             for (int i = 0; i < kLoad; ++i)
                 if (c + i == y) zt = u2f(r[i]);
         }
-        const float b = mn > -INFINITY ? mn * kLog2e : 0.f;  // -inf throughout, or NaN (which a maximum skips)
+        const float b = mn > -INFINITY ? mn * p.log2e : 0.f;  // -inf throughout, or NaN (which a maximum skips)
 #pragma unroll
         for (int i = 0; i < kLoad; i += 4)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s4[k] += ex2(fmaf(u2f(r[i + k]), kLog2e, -b));
-        s = s * ex2(fmaf(m, kLog2e, -b)) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+            for (int k = 0; k < 4; ++k) s4[k] += ex2(fmaf(u2f(r[i + k]), p.log2e, -b));
+        s = s * ex2(fmaf(m, p.log2e, -b)) + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
         m = mn;
     });
     if (row < p.T) {
-        p.part[static_cast<int64_t>(n0 / kPiece) * p.T + row] = make_float2(m, s);
-        if (y >= 0 && y < kPiece && y + n0 < p.V) p.zt[row] = zt;
+        p.part[static_cast<int64_t>(n0 / kPiece) * p.T + row] = make_float2(m * p.unbias, s);
+        if (y >= 0 && y < kPiece && y + n0 < p.V) p.zt[row] = zt * p.unbias;
     }
 }
 
-// dz of one piece: r_t (exp(z - lse) - [v = target]), r_t in the exponent where it is the same for all rows.
+// dz of one piece: r_t (exp(z - lse) - [v = target]) 2^15, the power of two in the exponent.
 template <bool BF16, class Release>
 __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t tacc, int64_t row, int row0, int n0,
                                        uint32_t stage, int lane, Release release) {
@@ -211,8 +212,8 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
     const int64_t y = target - t.v0 - n0;
     const float l2 = live ? p.lse[row] * kLog2e : 0.f;
     const bool own = p.row_scale != nullptr;
-    const float rs = !live ? 0.f : own ? p.row_scale[row] : (target != p.ignore_index ? p.unit : 0.f);
-    const float shift = own ? -l2 : p.log2_unit - l2;
+    const float rt = !live ? 0.f : own ? p.row_scale[row] : (target != p.ignore_index ? 1.f : 0.f);
+    const float shift = p.log2_unit - l2;
     each_load(tacc, release, [&](uint32_t* r, int c) {
         const bool hit = __any_sync(0xffffffffu, y >= c && y < c + kLoad);
 #pragma unroll
@@ -221,10 +222,10 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
             if (col < t.padded) {
                 uint32_t* q = r + b;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(ex2(fmaf(u2f(q[i]), kLog2e, shift)));
+                for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(ex2(fmaf(u2f(q[i]), p.log2e, shift)));
                 if (own) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(rs * u2f(q[i]));
+                    for (int i = 0; i < 32; ++i) q[i] = __float_as_uint(rt * u2f(q[i]));
                 }
                 if (col + 32 > t.N) {  // columns past the piece, which are read as K: zeros
 #pragma unroll
@@ -234,13 +235,13 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
                 if (hit) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (c + b + i == y) q[i] = __float_as_uint(u2f(q[i]) - rs);
+                        if (c + b + i == y) q[i] = __float_as_uint(fmaf(-rt, p.unit, u2f(q[i])));
                 }
                 uint32_t x[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     x[i] = pack2<BF16>(u2f(q[2 * i]), u2f(q[2 * i + 1]));
-                    if (rs == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
+                    if (rt == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
                 }
                 stage_box(stage, lane, x);
                 if (lane == 0 && row0 < t.M) {
@@ -863,8 +864,8 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const Rowwise 
     if (threadIdx.x == 0) *loss = static_cast<float>(p.reduction == MORPHO_REDUCTION_MEAN ? l / fmax(kept, 1.0) : l);
 }
 
-// Per-token gradients, one block: splits g_t into the factor that dz carries (row_scale = r_t unit) and
-// the common one of the results (*common = gmax / unit).
+// Per-token gradients, one block: splits g_t into the factor that dz carries (row_scale = r_t) and the
+// common one of the results (*common = gmax / unit).
 __global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, float* row_scale) {
     __shared__ float top[32];
     pdl_release();
@@ -883,7 +884,7 @@ __global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, floa
     if (most == 0.f) most = 1.f;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < p.T; i += 1024)
-        row_scale[i] = p.target[i] != p.ignore_index ? p.grad[i] / most * p.unit : 0.f;
+        row_scale[i] = p.target[i] != p.ignore_index ? p.grad[i] / most : 0.f;
     if (threadIdx.x == 0) *p.common = most / p.unit;
 }
 
@@ -1128,8 +1129,17 @@ int launch_join(const Rowwise& r, const FwdPlan& f, float* loss, float* lse, cud
     return MORPHO_OK;
 }
 
+// The tensor core truncates its fp32 accumulator after every K = 16 step: on average half a unit in the last
+// place of the running sum is lost, always towards zero.  For a sum that grows evenly to z in n steps these
+// units average 0.35 2^-23 z, so z comes out short by n 2.1e-8 of itself (measured 1.5e-8 in bf16, where
+// early sums are exact, and 1.9e-8 in fp16); 1.8e-8 is put back.  At dim 1024 that takes the error of a
+// target's logit from 8e-6 to that of an fp32 sum, 3e-6.
+float unbias_of(int dim) { return static_cast<float>(1.0 + (dim + 15) / 16 * 1.8e-8); }
+
 Rowwise rows_of(const morpho_vocab_loss_t* p, const int64_t* target) {
     Rowwise r{};
+    r.unbias = unbias_of(p->dim);
+    r.log2e = static_cast<float>(1.4426950408889634 * (1.0 + (p->dim + 15) / 16 * 1.8e-8));
     r.T = p->tokens;
     r.V = p->vocab;
     r.target = target;

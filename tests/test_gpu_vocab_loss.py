@@ -113,6 +113,21 @@ def test_many_tiles(cuda, T, V, D):
     check(*make(T, V, D, torch.bfloat16), reduction="none")
 
 
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("D", [256, 1024, 2048])
+def test_logits_are_not_biased(cuda, D, kind):
+    """The tensor core loses up to 2.1e-8 of a sum at each of its D / 16 steps, always towards zero; what is
+    put back leaves at most a third of that on average, beside the random part of an fp32 sum (2^-24 of the
+    result for the root of the steps, averaged over the tokens)."""
+    h, w, y = make(400, 3000, D, kind, ignored=0.0)
+    h = (h.float() + w[y].float()).to(kind)
+    loss, lse = M.linear_cross_entropy_forward(h, w, y, IGNORE, "none")
+    zt = (h.double() * w.double()[y]).sum(1)
+    short = (zt - (lse.double() - loss.double())) / zt
+    steps = D / 16
+    assert abs(short.mean().item()) <= steps * 2.1e-8 / 3 + 3 * steps ** 0.5 * 2.0 ** -24 / 400 ** 0.5 + 2.0 ** -23
+
+
 def test_gradients_of_very_different_rows(cuda):
     """Row gradients over eight orders of magnitude, zeros and negative ones among them."""
     h, w, y = make(64, 300, 64, torch.bfloat16, ignored=0.0)
