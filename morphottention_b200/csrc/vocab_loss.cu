@@ -244,7 +244,7 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
                     if (rt == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
                 }
                 stage_box(stage, lane, x);
-                if (lane == 0 && row0 < t.M) {
+                if (lane == 0) {
                     tma_store_2d(&t.out, stage, col, row0);
                     bulk_commit_group();
                 }
@@ -266,7 +266,7 @@ __device__ __forceinline__ void epi_out(const Rowwise& p, const Task& t, uint32_
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[i] = pack2<BF16>(g * u2f(r[b + 2 * i]), g * u2f(r[b + 2 * i + 1]));
                 stage_box(stage, lane, x);
-                if (lane == 0 && row0 < t.M) {
+                if (lane == 0) {
                     tma_store_2d(&t.out, stage, n0 + c + b, row0);
                     bulk_commit_group();
                 }
@@ -284,7 +284,7 @@ __device__ __forceinline__ void epi_part(const Task& t, uint32_t tacc, int row0,
         for (int b = 0; b < kLoad; b += 16) {
             if (n0 + c + b < t.N) {
                 stage_box(stage, lane, r + b);
-                if (lane == 0 && row0 < t.M) {
+                if (lane == 0) {
                     if (t.kind == kPartAdd)
                         tma_reduce_add_3d(&t.out, stage, n0 + c + b, row0, z);
                     else
@@ -586,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * a, 0));
             };
-            if (n0 >= t.N) {  // (dz: its padding ends inside the last live piece)
+            if (n0 >= t.N || row0 >= t.M) {  // (dz: its padding ends inside the last live piece)
                 release();
             } else if (t.kind == kStats) {
                 epi_stats(L.rows, tacc, static_cast<int64_t>(row0) + lane, n0, release);
@@ -1067,6 +1067,15 @@ int add_task(Launch* L, Task& t, int kind, bool a_mn, bool b_mn, int64_t M, int6
     return MORPHO_OK;
 }
 
+// Whether a launch's tiles are taken from a counter as pairs become free, rather than dealt round-robin: an
+// item takes 2 us to reach all roles of a pair, which tiles of a few K blocks (0.5 us each) hide and shorter ones do not
+// (backward of 3 tokens, 32768 x 1024: 69 us dealt, 72 taken; of 200, 65536 x 2048, 3.6 blocks a tile: 239 and 222).
+bool worth_taking(const Launch& L) {
+    int64_t units = 0;
+    for (int i = 0; i < L.tasks; ++i) units += static_cast<int64_t>(L.task[i].tiles_m) * L.task[i].tiles_n * L.task[i].k_blocks;
+    return units >= 3LL * L.task[L.tasks - 1].items_end;
+}
+
 template <bool BF16>
 int launch(const DeviceInfo& dev, Launch& L, cudaStream_t stream, const char* name) {
     auto kern = vocab_gemm_kernel<BF16>;
@@ -1193,6 +1202,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
     for (int i = -1; i < c.pieces; ++i) {
         Launch L{};
         L.rows = r;
+        bool mixed = false;  // tiles of different lengths
         if (i >= 0) L.rows.grad = nullptr;  // the first launch makes *common
         if (i >= 0) {
             const int v0 = i * c.cols;
@@ -1221,7 +1231,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
             const bool h_first = ceil_div(n, splits_h) > ceil_div(T, c.splits_w);
             MORPHO_TRY(h_first ? add_h() : add_w());
             MORPHO_TRY(h_first ? add_w() : add_h());
-            L.next = f.next + i;
+            mixed = true;
         } else {
             L.zero = f.next;
             L.zeros = c.pieces;
@@ -1236,6 +1246,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
             MORPHO_TRY(store_map(&z.out, f.dz[(i + 1) & 1], T, z.padded, c.cols));
             MORPHO_TRY(add_task(&L, z, kDz, false, false, T, width(i + 1), D, 1));
         }
+        if (mixed && worth_taking(L)) L.next = f.next + i;
         MORPHO_TRY(launch<BF16>(dev, L, stream, i < 0 ? "vocab_dz" : "vocab_grad"));
         if (i >= 0 && c.splits_w > 1)
             MORPHO_TRY(finish<BF16>(dev, f.wpart, c.splits_w, width(i) * D, f.common,
