@@ -423,6 +423,67 @@ def peer_destroy(group: int) -> None:
     _check(lib().morpho_sm100_peer_destroy(group))
 
 
+_DTYPES = {"torch.float16": MORPHO_DTYPE_F16, "torch.bfloat16": MORPHO_DTYPE_BF16, "torch.float32": MORPHO_DTYPE_F32}
+
+
+def _dtype(t) -> int:
+    return _DTYPES[str(t.dtype)]
+
+
+def _workspace(nbytes: int, like):
+    import torch
+    if nbytes == 0:
+        raise MorphoError(MORPHO_ERR_INVALID, last_error())
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def layer_norm_problem(x, weight=None, eps: float = 1e-5) -> MorphoLayerNorm:
+    """The problem of contiguous ``x`` ``[rows, dim]``."""
+    return MorphoLayerNorm(x.shape[0], x.shape[1], _dtype(x), _dtype(x if weight is None else weight), eps, 0, 0, 0, 0)
+
+
+def layer_norm_forward(p: MorphoLayerNorm, x, residual, weight, bias, y, h, mean, rstd, stream=None) -> None:
+    _check(lib().morpho_sm100_layer_norm_forward(ctypes.byref(p), _ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y),
+                                                 _ptr(h), _ptr(mean), _ptr(rstd), _stream(stream)))
+
+
+def layer_norm_backward(p: MorphoLayerNorm, grad_y, grad_h, h, weight, mean, rstd, dx, dweight, dbias,
+                        stream=None) -> None:
+    ws = _workspace(lib().morpho_sm100_layer_norm_backward_workspace_size(ctypes.byref(p)), h)
+    _check(lib().morpho_sm100_layer_norm_backward(ctypes.byref(p), _ptr(grad_y), _ptr(grad_h), _ptr(h), _ptr(weight),
+                                                  _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(ws),
+                                                  ws.numel(), _stream(stream)))
+
+
+def vocab_loss_problem(hidden, weight, ignore_index: int = -100, reduction: str = "mean") -> MorphoVocabLoss:
+    """The problem of contiguous ``hidden`` ``[tokens, dim]`` and ``weight`` ``[vocab, dim]``."""
+    return MorphoVocabLoss(hidden.shape[0], weight.shape[0], hidden.shape[1], _dtype(hidden), REDUCTIONS[reduction],
+                           ignore_index, 0, 0)
+
+
+def linear_cross_entropy_forward(p: MorphoVocabLoss, hidden, weight, target, loss, lse, stream=None) -> None:
+    ws = _workspace(lib().morpho_sm100_linear_cross_entropy_forward_workspace_size(ctypes.byref(p)), hidden)
+    _check(lib().morpho_sm100_linear_cross_entropy_forward(ctypes.byref(p), _ptr(hidden), _ptr(weight), _ptr(target),
+                                                           _ptr(loss), _ptr(lse), _ptr(ws), ws.numel(), _stream(stream)))
+
+
+def linear_cross_entropy_backward(p: MorphoVocabLoss, grad_loss, hidden, weight, target, lse, dhidden, dweight,
+                                  stream=None) -> None:
+    ws = _workspace(lib().morpho_sm100_linear_cross_entropy_backward_workspace_size(ctypes.byref(p)), hidden)
+    _check(lib().morpho_sm100_linear_cross_entropy_backward(ctypes.byref(p), _ptr(grad_loss), _ptr(hidden), _ptr(weight),
+                                                            _ptr(target), _ptr(lse), _ptr(dhidden), _ptr(dweight), _ptr(ws),
+                                                            ws.numel(), _stream(stream)))
+
+
+def clip_grad_norm(grads, out, max_norm: float, norm, loss_scale: float = 1.0, stream=None) -> None:
+    """Contiguous ``grads`` into ``out`` (one list of tensors each), their norm into the fp32 ``norm``."""
+    pairs = (MorphoTensorPair * max(1, len(grads)))(*(MorphoTensorPair(_ptr(g), _ptr(o), g.numel(), _dtype(g), _dtype(o))
+                                                      for g, o in zip(grads, out)))
+    ws = _workspace(lib().morpho_sm100_clip_grad_norm_workspace_size(len(grads)), norm)
+    _check(lib().morpho_sm100_clip_grad_norm(pairs, len(grads), max_norm, loss_scale, _ptr(norm), _ptr(ws), ws.numel(),
+                                             _stream(stream)))
+
+
 def score_probe_half2(qc, kc, rowmax, stream=None) -> None:
     """Row maxima of qc . k^T over all keys on packed half2 CUDA-core math (the design probe
     ``morpho_sm100_score_probe_half2``); qc, kc fp16 [BH, N, m], rowmax fp32 [BH, N]."""
