@@ -203,7 +203,7 @@ __device__ __forceinline__ void segment_scale(const T* p, O* q, int n, float by,
 
 template <class Tab>
 __global__ void __launch_bounds__(kThreads, kScalePerSm)
-    grad_scale_kernel(const __grid_constant__ Tab t, const double* part, int parts, float max_norm, float inv_scale,
+    grad_scale_kernel(const __grid_constant__ Tab t, const double* part, int parts, float max_norm, float loss_scale,
                       float* norm_out) {
     extern __shared__ __align__(16) uint8_t stages[];
     __shared__ double scratch[kWarps];
@@ -212,11 +212,12 @@ __global__ void __launch_bounds__(kThreads, kScalePerSm)
     double sum = 0.0;
     for (int i = threadIdx.x; i < parts; i += kThreads) sum += part[i];
     sum = block_sum(sum, scratch);
-    const float norm = static_cast<float>(sqrt(sum) * static_cast<double>(inv_scale));
-    float c = max_norm / (norm + 1e-6f);
-    c = c > 1.0f ? 1.0f : c;  // NaN stays NaN
-    if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
-    const float by = c * inv_scale;
+    // in fp64 to the factor itself, which is then one rounding away
+    const double norm = sqrt(sum) / loss_scale;
+    double c = max_norm / (norm + 1e-6);
+    c = c > 1.0 ? 1.0 : c;  // NaN stays NaN
+    if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = static_cast<float>(norm);
+    const float by = static_cast<float>(c / loss_scale);
     uint8_t* stage = stages + (threadIdx.x >> 5) * kStageBytes;
     for (int k = blockIdx.x; k < t.chunks; k += gridDim.x) {
         const int i = tensor_of(t, k);
@@ -265,7 +266,7 @@ int64_t fill(Table<N>* t, const morpho_tensor_pair_t* pairs, int64_t first, int6
 
 // Both passes, with tables of up to N tensors.
 template <int N>
-int clip(const DeviceInfo& dev, const morpho_tensor_pair_t* pairs, int64_t count, float max_norm, float inv_scale, float* norm, double* part,
+int clip(const DeviceInfo& dev, const morpho_tensor_pair_t* pairs, int64_t count, float max_norm, float loss_scale, float* norm, double* part,
          int64_t limit, cudaStream_t stream) {
     auto scale = grad_scale_kernel<Table<N>>;
     constexpr int smem = kWarps * kStageBytes;
@@ -288,7 +289,7 @@ int clip(const DeviceInfo& dev, const morpho_tensor_pair_t* pairs, int64_t count
         if (launches > 1) i = fill(&t, pairs, i, count);
         const int blocks = std::max(1, std::min(t.chunks, kScalePerSm * dev.sms));
         prof_begin(stream, "grad_scale");
-        MORPHO_CUDA_TRY(launch_after(scale, blocks, kThreads, smem, stream, t, part, static_cast<int>(parts), max_norm, inv_scale, k == 0 ? norm : nullptr));
+        MORPHO_CUDA_TRY(launch_after(scale, blocks, kThreads, smem, stream, t, part, static_cast<int>(parts), max_norm, loss_scale, k == 0 ? norm : nullptr));
         MORPHO_LAUNCH_CHECK("grad_scale");
     }
     return MORPHO_OK;
@@ -340,9 +341,8 @@ extern "C" MORPHO_API int morpho_sm100_clip_grad_norm(const morpho_tensor_pair_t
         return set_error(MORPHO_ERR_WORKSPACE, "clip workspace too small: %zu bytes", workspace_bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* part = static_cast<double*>(workspace);
-    const float inv_scale = 1.0f / loss_scale;
     const int64_t limit = static_cast<int64_t>(workspace_bytes / sizeof(double));
-    return count <= kFewTensors    ? clip<kFewTensors>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st)
-           : count <= kSomeTensors ? clip<kSomeTensors>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st)
-                                   : clip<kTable>(dev, pairs, count, max_norm, inv_scale, norm, part, limit, st);
+    return count <= kFewTensors    ? clip<kFewTensors>(dev, pairs, count, max_norm, loss_scale, norm, part, limit, st)
+           : count <= kSomeTensors ? clip<kSomeTensors>(dev, pairs, count, max_norm, loss_scale, norm, part, limit, st)
+                                   : clip<kTable>(dev, pairs, count, max_norm, loss_scale, norm, part, limit, st);
 }
