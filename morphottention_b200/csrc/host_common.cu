@@ -206,6 +206,13 @@ int make_tmap_2d_f32(CUtensorMap* map, const void* base, uint64_t rows, uint64_t
 int current_device_info(DeviceInfo* out) {
     int dev = 0;
     MORPHO_CUDA_TRY(cudaGetDevice(&dev));
+    // A thread's first call: make the device's context current on it.  The tensor maps are encoded by the driver,
+    // which fails without one, and nothing before it need have touched the device (autograd's worker thread).
+    static thread_local int bound = -1;
+    if (bound != dev) {
+        MORPHO_CUDA_TRY(cudaSetDevice(dev));
+        bound = dev;
+    }
     if (dev < 0 || dev >= kMaxDevices) return set_error(MORPHO_ERR_DEVICE, "device ordinal %d out of range", dev);
     std::lock_guard<std::mutex> lock(g_info_mu);
     DeviceInfo& info = g_info[dev];

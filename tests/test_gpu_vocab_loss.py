@@ -6,6 +6,8 @@ probabilities inherit it (plus a few 2^-22 of their own).  dz is rounded once to
 itself; 2^-40 below fp16's range), the products' fp32 sums add (terms / 16) 2^-23 of their magnitudes,
 and the result is rounded once."""
 
+import threading
+
 import pytest
 import torch
 
@@ -282,6 +284,19 @@ def test_autograd(cuda):
     h.grad = None
     M.linear_cross_entropy(h, w, y, reduction="sum").backward()
     assert torch.equal(a, h.grad)
+
+
+def test_first_call_of_a_thread(cuda):
+    """A thread that has not used the device yet, as autograd's worker when the loss is what backward starts from."""
+    h, w, y = make(64, 300, 128, torch.float16)
+    one = torch.ones((), device="cuda")
+    _, lse = M.linear_cross_entropy_forward(h, w, y)
+    want = [t.clone() for t in M.linear_cross_entropy_backward(one, h, w, y, lse)]
+    got = []
+    t = threading.Thread(target=lambda: got.extend(M.linear_cross_entropy_backward(one, h, w, y, lse)))
+    t.start()
+    t.join()
+    assert len(got) == 2 and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_on_another_stream_and_captured(cuda):
