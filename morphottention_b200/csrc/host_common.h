@@ -86,7 +86,9 @@ cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned block, si
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (e != cudaSuccess) cudaGetLastError();  // reported by the caller, not left for the next launch check
+    return e;
 }
 
 // Tiled tensor map over a row-major fp16/fp32 tensor.  dims/box are innermost first;

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from ._ops import add_op_namespace_prefix, ops
 
@@ -84,6 +85,7 @@ class LayerNormFunction(torch.autograd.Function):
         return (y, h[0]) if h else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_y, grad_h=None):
         h, weight, mean, rstd = ctx.saved_tensors
         if grad_y is None:  # only h was used
@@ -163,6 +165,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_loss):
         hidden, weight, target, lse = ctx.saved_tensors
         dh, dw = _loss_backward(grad_loss, hidden, weight, target, lse, *ctx.options)

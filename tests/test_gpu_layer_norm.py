@@ -285,6 +285,14 @@ def test_autograd_module_and_residual(cuda):
     assert x.grad is not None
 
 
+def test_no_second_derivative(cuda):
+    x = torch.randn(4, 64, device="cuda", requires_grad=True)
+    one = torch.ones(64, device="cuda")
+    (dx,) = torch.autograd.grad(M.layer_norm(x, one, one).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
 def test_on_another_stream(cuda):
     d = make(64, 512, torch.float16, torch.float16, residual=True)
     want = M.layer_norm_forward(d["x"], d["w"], d["b"], EPS, d["res"])

@@ -140,6 +140,14 @@ def test_gradients_of_very_different_rows(cuda):
     check(h, w, y, "none", torch.zeros(64, device="cuda"))
 
 
+def test_no_second_derivative(cuda):
+    h, w, y = make(16, 40, 64, torch.float16)
+    h.requires_grad_()
+    (dh,) = torch.autograd.grad(M.linear_cross_entropy(h, w, y).square(), h, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dh.float().sum().backward()
+
+
 def test_all_ignored(cuda):
     for reduction, grad in (("none", torch.ones(40, device="cuda")), ("mean", torch.ones((), device="cuda")),
                             ("sum", torch.ones((), device="cuda"))):
