@@ -22,6 +22,7 @@
 // MMA issuer (rank 0 of the pair), warps 2-17 epilogue, warp 18 scheduler; the accumulator is double-buffered in TMEM, and
 // results leave through TMA stores from a swizzled box per warp.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "elem.cuh"
@@ -48,7 +49,8 @@ constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kBoxBytes = 2048;                      // of an epilogue warp's stores: 32 rows of 64 bytes
 constexpr int kStoreOffset = kStages * kStageBytes;  // a box for each of them
 constexpr int kBarOffset = kStoreOffset + kEpiWarps * kBoxBytes;
-constexpr int kSmemBytes = kBarOffset + 512 + 1024;
+constexpr int kBarBytes = 256;  // the barriers, then as much for the epilogue's sums
+constexpr int kSmemBytes = kBarOffset + 2 * kBarBytes + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory");
 
 // What a GEMM's epilogue does with its tile.
@@ -103,9 +105,9 @@ struct Rowwise {
     uint32_t* done; // forward: the join kernel's count of finished blocks
     const float* lse;
     const float* grad;
-    const float* row_scale;  // r_t (0 for ignored rows); NULL: 1, or 0
     float unit, log2_unit;
-    float* common;  // gmax / unit, the factor of the results
+    bool first;     // backward: this launch makes *common
+    float* common;  // gmax / unit, the factor of the results; g_t = gmax r_t
 };
 
 constexpr int kMaxTasks = 3;
@@ -206,13 +208,13 @@ __device__ __forceinline__ void epi_stats(const Rowwise& p, uint32_t tacc, int64
 // dz of one piece: r_t (exp(z - lse) - [v = target]) 2^15, the power of two in the exponent.
 template <bool BF16, class Release>
 __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t tacc, int64_t row, int row0, int n0,
-                                       uint32_t stage, int lane, Release release) {
+                                       uint32_t stage, int lane, float top, Release release) {
     const bool live = row < p.T;
     const int64_t target = live ? p.target[row] : -1;
     const int64_t y = target - t.v0 - n0;
     const float l2 = live ? p.lse[row] * kLog2e : 0.f;
-    const bool own = p.row_scale != nullptr;
-    const float rt = !live ? 0.f : own ? p.row_scale[row] : (target != p.ignore_index ? 1.f : 0.f);
+    const bool own = p.reduction == MORPHO_REDUCTION_NONE;
+    const float rt = !live || target == p.ignore_index ? 0.f : own ? p.grad[row] / top : 1.f;
     const float shift = p.log2_unit - l2;
     each_load(tacc, release, [&](uint32_t* r, int c) {
         const bool hit = __any_sync(0xffffffffu, y >= c && y < c + kLoad);
@@ -370,6 +372,24 @@ struct Items {
     }
 };
 
+// The largest finite |g_t| of the rows that are not ignored (1 if there is none), by the epilogue's threads.  At least
+// unit x FLT_MIN, so that the later launches get the same value back from *common.
+__device__ __forceinline__ float largest_gradient(const Rowwise& p, float* scratch, int thread) {
+    float most = 0.f;
+#pragma unroll 4
+    for (int64_t i = thread; i < p.T; i += 32 * kEpiWarps) {
+        const float g = fabsf(p.grad[i]);
+        if (p.target[i] != p.ignore_index && isfinite(g)) most = fmaxf(most, g);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((thread & 31) == 0) scratch[thread >> 5] = most;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+#pragma unroll
+    for (int i = 0; i < kEpiWarps; ++i) most = fmaxf(most, scratch[i]);
+    return most > 0.f ? fmaxf(most, p.unit * FLT_MIN) : 1.f;
+}
+
 // One operand of a stage: rows (M or N) x .. x + 127, K k .. k + 127, in two panels of 128 rows of 128 bytes.
 // K-major: the panels are the halves of K; MN-major: the halves of the rows, each with K down.
 __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap& map, uint32_t bar, bool mn, bool whole, int row0,
@@ -397,7 +417,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
     // full, empty, acc_full[2], acc_empty[2], drain, item full, item empty
     constexpr int NB = 2 * kStages + 5 + 2 * kSlots;
     constexpr int kSlotWord = (NB * 8 + 8 + 15) / 16 * 4;  // first word of the item ring, after the two below
-    static_assert(kSlotWord * 4 + 16 * kSlots <= 512, "barrier block");
+    static_assert(kSlotWord * 4 + 16 * kSlots <= kBarBytes, "barrier block");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     const int warp = warp_id();
@@ -533,7 +553,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
             }
         }
         // One idle warp counts the rows of a mean for the launches that scale results by it.
-        if (blockIdx.x == 1 && L.rows.grad != nullptr && L.rows.row_scale == nullptr) {
+        if (blockIdx.x == 1 && L.rows.first && L.rows.reduction != MORPHO_REDUCTION_NONE) {
             int64_t kept = 0;
             if (L.rows.reduction == MORPHO_REDUCTION_MEAN) {
 #pragma unroll 8
@@ -561,6 +581,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
         // ---------------- epilogue, in both CTAs ----------------
         const int set = (warp - 2) / kSetWarps, quad = warp & 3, piece = ((warp - 2) >> 2) & 1;
         const uint32_t stage = smem_u32(smem + kStoreOffset + (warp - 2) * kBoxBytes);
+        // Per-token gradients: the largest of them.  The first launch looks for itself, in every CTA (a few us
+        // beside the first tile's loads), and leaves it to the others.
+        float top = 1.f;
+        if (L.rows.reduction == MORPHO_REDUCTION_NONE && L.rows.grad != nullptr) {
+            if (L.rows.first) {
+                top = largest_gradient(L.rows, reinterpret_cast<float*>(smem + kBarOffset + kBarBytes), threadIdx.x - 64);
+                if (blockIdx.x == 0 && threadIdx.x == 64) *L.rows.common = top / L.rows.unit;
+            } else {
+                top = *L.rows.common * L.rows.unit;
+            }
+        }
         Item it = item_of(L, first);
         for (int j = set;; j += 2) {  // set 0 the even items, set 1 the odd ones
             if (j > 0) {
@@ -591,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
             } else if (t.kind == kStats) {
                 epi_stats(L.rows, tacc, static_cast<int64_t>(row0) + lane, n0, release);
             } else if (t.kind == kDz) {
-                epi_dz<BF16>(L.rows, t, tacc, static_cast<int64_t>(row0) + lane, row0, n0, stage, lane, release);
+                epi_dz<BF16>(L.rows, t, tacc, static_cast<int64_t>(row0) + lane, row0, n0, stage, lane, top, release);
             } else if (t.kind == kOut) {
                 epi_out<BF16>(L.rows, t, tacc, row0, n0, stage, lane, release);
             } else {
@@ -864,30 +895,6 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const Rowwise 
     if (threadIdx.x == 0) *loss = static_cast<float>(p.reduction == MORPHO_REDUCTION_MEAN ? l / fmax(kept, 1.0) : l);
 }
 
-// Per-token gradients, one block: splits g_t into the factor that dz carries (row_scale = r_t) and the
-// common one of the results (*common = gmax / unit).
-__global__ void __launch_bounds__(1024) vocab_scale_kernel(const Rowwise p, float* row_scale) {
-    __shared__ float top[32];
-    pdl_release();
-    pdl_wait();
-    float most = 0.f;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < p.T; i += 1024) {
-        const float g = fabsf(p.grad[i]);
-        if (p.target[i] != p.ignore_index && isfinite(g)) most = fmaxf(most, g);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = most;
-    __syncthreads();
-    for (int i = 0; i < 32; ++i) most = fmaxf(most, top[i]);
-    if (most == 0.f) most = 1.f;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < p.T; i += 1024)
-        row_scale[i] = p.target[i] != p.ignore_index ? p.grad[i] / most : 0.f;
-    if (threadIdx.x == 0) *p.common = most / p.unit;
-}
-
 // ---- host ---------------------------------------------------------------------------------------
 
 constexpr size_t kPieceBytes = 512u << 20;  // dz of one piece of the vocabulary, at most; two are held
@@ -996,7 +1003,7 @@ void plan_forward(Bump& b, const morpho_vocab_loss_t* p, int sms, FwdPlan* f) {
 struct BwdPlan {
     Cut cut;
     uint16_t* dz[2];
-    float *row_scale, *common, *hpart, *wpart;
+    float *common, *hpart, *wpart;
     uint32_t* next;  // a work counter for each launch after the first
 };
 void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
@@ -1004,7 +1011,6 @@ void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
     const Cut& c = f->cut;
     const size_t T = p->tokens, D = p->dim;
     for (int i = 0; i < 2; ++i) f->dz[i] = b.take<uint16_t>(i < c.pieces ? T * c.cols : 0);
-    f->row_scale = b.take<float>(T);
     f->common = b.take<float>(1);
     f->next = b.take<uint32_t>(c.pieces);
     f->hpart = b.take<float>(c.pieces > 1 || c.splits_h > 1 ? c.splits_h * T * D : 0);
@@ -1190,12 +1196,6 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
     r.unit = BF16 ? 1.0f : 32768.0f;
     r.log2_unit = BF16 ? 0.0f : 15.0f;
     r.common = f.common;
-    if (p->reduction == MORPHO_REDUCTION_NONE) {
-        prof_begin(stream, "vocab_scale");
-        MORPHO_CUDA_TRY(launch_after(vocab_scale_kernel, 1, 1024, 0, stream, r, f.row_scale));
-        MORPHO_LAUNCH_CHECK("vocab_scale");
-        r.row_scale = f.row_scale;
-    }
     const Cut& c = f.cut;
     const int64_t T = p->tokens, D = p->dim;
     auto width = [&](int i) { return std::min<int64_t>(c.cols, p->vocab - static_cast<int64_t>(i) * c.cols); };
@@ -1203,7 +1203,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
         Launch L{};
         L.rows = r;
         bool mixed = false;  // tiles of different lengths
-        if (i >= 0) L.rows.grad = nullptr;  // the first launch makes *common
+        L.rows.first = i < 0;
         if (i >= 0) {
             const int v0 = i * c.cols;
             const int64_t n = width(i), padded = ceil_div(n, 64) * 64;  // dz holds zeros up to whole panels

@@ -140,6 +140,21 @@ def test_gradients_of_very_different_rows(cuda):
     check(h, w, y, "none", torch.zeros(64, device="cuda"))
 
 
+@pytest.mark.parametrize("kind,tokens", [(torch.bfloat16, 40), (torch.float16, 40), (torch.float16, (1 << 20) + 77)])
+def test_gradients_below_the_normal_range(cuda, kind, tokens):
+    """2^-140 a row: below fp32's normal numbers, so the gradients stay within sum |dz| max |operand| of
+    zero (sum over v of |dz| is at most 2 g, each |dz| at most g).  The many tokens make two pieces of dz."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    h = torch.randn(tokens, 8, generator=g, device="cuda").to(kind)
+    w = torch.randn(300, 8, generator=g, device="cuda").to(kind)
+    y = torch.randint(0, 300, (tokens,), generator=g, device="cuda")
+    grad = torch.full((tokens,), 2.0 ** -140, device="cuda")
+    _, lse = M.linear_cross_entropy_forward(h, w, y, IGNORE, "none")
+    dh, dw = M.linear_cross_entropy_backward(grad, h, w, y, lse, IGNORE, "none")
+    assert dh.double().abs().max() <= 2 * w.double().abs().max() * 2.0 ** -140
+    assert dw.double().abs().max() <= tokens * h.double().abs().max() * 2.0 ** -140
+
+
 def test_no_second_derivative(cuda):
     h, w, y = make(16, 40, 64, torch.float16)
     h.requires_grad_()
