@@ -7,9 +7,11 @@
 // it still holds.  A norm that is not finite makes the gradients non-finite (0 * inf, NaN), as dividing
 // by it does.
 //
-// The tensors are cut into chunks, dealt to a persistent grid, of one 2 KB segment for each warp.  The table of tensors travels as a kernel parameter, so a launch needs no copy to the device
-// and can be captured in a graph.  (Taking the chunks in reverse in the second pass, to find in L2 what the
-// first read last, and storing with low cache priority changed nothing: 69 us each for 390 MB.)
+// The tensors are cut into chunks, dealt to a persistent grid, of one 2 KB segment for each warp.  The table
+// of tensors travels as a kernel parameter, so a launch needs no copy to the device and can be captured in a
+// graph.  Measured: 144 tensors, 65M fp16 values to fp32, 96 us (5.5 TB/s with the second read); 36 tensors of
+// odd sizes, 7.2M bf16, 13 us in the kernels.  (Taking the chunks in reverse in the second pass, to
+// find in L2 what the first read last, and storing with low cache priority changed nothing: 69 us each for 390 MB.)
 //
 // Alignment: a segment is read as the aligned 16-byte packs that cover it, with the neighbours' elements in
 // the first and the last masked.  Where input and output stand differently to a 16-byte boundary the
