@@ -10,6 +10,7 @@ the losses.
 from __future__ import annotations
 
 import argparse
+import math
 
 import torch
 from torch import nn
@@ -79,8 +80,10 @@ class CausalLanguageModel(nn.Module):
 class MixedPrecisionStep:
     """Training steps of a float16 model with float32 master weights: the loss is multiplied by
     ``loss_scale``, the gradients are brought to float32 and clipped to ``max_norm`` in one operator, an
-    optimizer updates the masters, and the model's weights are copied from them.  A step whose gradients
-    are not finite changes nothing (the skip happens on the device; nothing waits on the host).
+    optimizer updates the masters, and the model's weights are copied from them.  A step whose gradient
+    norm is not finite changes nothing: masters, weights and the optimizer's state keep their values.
+    (The optimizer is not called then, since zero gradients would still move what has momentum or weight
+    decay; so the host reads the norm, and waits for the backward pass, once a step.)
 
     :param make_optimizer: builds the optimizer from the list of masters.
     :returns: ``step(tokens, targets)`` gives ``(loss, gradient norm)``, tensors on the device."""
@@ -100,12 +103,10 @@ class MixedPrecisionStep:
         (loss * self.loss_scale).backward()
         pairs = [(p.grad, m.grad) for p, m in zip(self.params, self.masters) if p.grad is not None]
         norm = clip_grad_norm([g for g, _ in pairs], self.max_norm, out=[g for _, g in pairs], loss_scale=self.loss_scale)
-        finite = torch.isfinite(norm)
-        for _, g in pairs:  # a skipped step has zero gradients
-            g.copy_(torch.where(finite, g, 0.0))
-        self.optimizer.step()
-        with torch.no_grad():
-            torch._foreach_copy_(self.params, self.masters)
+        if math.isfinite(norm.item()):
+            self.optimizer.step()
+            with torch.no_grad():
+                torch._foreach_copy_(self.params, self.masters)
         return loss.detach(), norm
 
 

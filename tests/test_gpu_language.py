@@ -107,3 +107,20 @@ def test_captured_forward_and_backward(cuda):
             assert (p.grad.double() - w.double()).norm() <= 1e-2 * w.double().norm()
         else:
             assert (p.grad.double() - w.double()).norm() <= 5e-3 * w.double().norm(), n
+
+
+def test_overflow_after_a_good_step_changes_nothing(cuda):
+    """With an optimizer that has momentum and weight decay, which zero gradients would still move."""
+    torch.manual_seed(3)
+    model = CausalLanguageModel(300, 64, 1, 16, 1, device="cuda")
+    step = MixedPrecisionStep(model, lambda ps: torch.optim.AdamW(ps, lr=1e-2), loss_scale=512.0)
+    step(*synthetic_batch(2, 20, 300, 0, cuda))
+
+    def everything():
+        state = [v for s in step.optimizer.state.values() for v in s.values()]
+        return [t.detach().clone() for t in (*model.parameters(), *step.masters, *state)]
+    before = everything()
+    step.loss_scale = 2.0 ** 40
+    _, norm = step(*synthetic_batch(2, 20, 300, 1, cuda))
+    assert not torch.isfinite(norm)
+    assert all(torch.equal(a, b) for a, b in zip(before, everything()))
