@@ -92,8 +92,7 @@ class MixedPrecisionStep:
         self.model, self.max_norm, self.loss_scale = model, max_norm, loss_scale
         self.params = [p for p in model.parameters() if p.requires_grad]
         self.masters = [p.detach().float().requires_grad_() for p in self.params]
-        for m in self.masters:
-            m.grad = torch.zeros_like(m)
+        self.grads = [torch.zeros_like(m) for m in self.masters]  # what the masters' gradients are written to
         self.optimizer = make_optimizer(self.masters)
 
     def __call__(self, *batch):
@@ -101,8 +100,10 @@ class MixedPrecisionStep:
         for p in self.params:
             p.grad = None
         (loss * self.loss_scale).backward()
-        pairs = [(p.grad, m.grad) for p, m in zip(self.params, self.masters) if p.grad is not None]
-        norm = clip_grad_norm([g for g, _ in pairs], self.max_norm, out=[g for _, g in pairs], loss_scale=self.loss_scale)
+        for p, m, g in zip(self.params, self.masters, self.grads):  # a parameter that took no part has no gradient
+            m.grad = None if p.grad is None else g
+        norm = clip_grad_norm([p.grad for p in self.params if p.grad is not None], self.max_norm,
+                              out=[m.grad for m in self.masters if m.grad is not None], loss_scale=self.loss_scale)
         if math.isfinite(norm.item()):
             self.optimizer.step()
             with torch.no_grad():

@@ -70,3 +70,16 @@ def test_a_step_that_is_not_finite_changes_nothing(step, good, bad):
     _, norm = step(torch.randn(5, 6))  # and the next one works again
     assert torch.isfinite(norm) and not same(before, everything(step))
     assert all(torch.isfinite(m).all() for m in step.masters)
+
+
+def test_a_parameter_without_a_gradient_is_left_alone(step):
+    step(torch.randn(5, 6))
+    alone = {id(p) for p in step.model.b.parameters()}
+    before = copy.deepcopy([(p.detach(), m.detach(), step.optimizer.state[m]) for p, m in zip(step.params, step.masters)])
+    x = torch.randn(5, 6)
+    _, norm = step(x, False)  # `b` takes no part
+    after = [(p.detach(), m.detach(), step.optimizer.state[m]) for p, m in zip(step.params, step.masters)]
+    for p, old, new in zip(step.params, before, after):
+        assert same(old, new) == (id(p) in alone)
+    _, norm = step(x)  # takes part again
+    assert all(m.grad is not None for m in step.masters)
