@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/morpho_sm100.h"
 
@@ -60,14 +61,18 @@ int prof_collect(char* names, int name_len, float* total_ms, int* counts, int ma
     } while (0)
 
 // Allow a kernel `bytes` of dynamic shared memory on the current device (one `set` per kernel: the call is
-// made when a device's first launch, or a larger one, needs it).
+// made when a device's first launch, or a larger one, needs it).  Checking, setting and recording hold a
+// lock, so that threads whose launches differ in size never lower the limit for one another.
 struct SharedLimit {
     std::atomic<int> set[64] = {};
+    std::mutex raising;
     template <class K>
     cudaError_t raise(K kernel, int device, int bytes) {
-        if (bytes <= 48 * 1024 || set[device].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
+        if (bytes <= 48 * 1024 || set[device].load(std::memory_order_acquire) >= bytes) return cudaSuccess;
+        const std::lock_guard<std::mutex> lock(raising);
+        if (set[device].load(std::memory_order_relaxed) >= bytes) return cudaSuccess;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) set[device].store(bytes, std::memory_order_relaxed);
+        if (e == cudaSuccess) set[device].store(bytes, std::memory_order_release);
         return e;
     }
 };
