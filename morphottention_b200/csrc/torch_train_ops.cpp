@@ -81,6 +81,7 @@ morpho_layer_norm_t norm_problem(const at::Tensor& x, const std::optional<at::Te
     TORCH_CHECK(x.dim() >= 1, name, " must have at least one dimension");
     const int64_t dim = x.size(x.dim() - 1);
     TORCH_CHECK(dim > 0, name, " must not have an empty last dimension");
+    TORCH_CHECK(dim <= INT32_MAX, name, " has too long a last dimension (", dim, ")");  // the problem holds 32 bits
     morpho_layer_norm_t p{};
     p.rows = x.numel() / dim;
     p.dim = static_cast<int32_t>(dim);

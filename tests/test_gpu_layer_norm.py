@@ -332,3 +332,12 @@ def test_refusals(cuda):
         M.layer_norm_backward(d["gy"], h, d["w"], mean[:2], rstd)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         f(d["x"], d["w"].cpu(), None)
+
+
+def test_last_dimension_past_32_bits_is_refused(cuda):
+    x = torch.zeros(1, device="cuda", dtype=torch.float16).expand((1 << 32) + 64)
+    one = torch.ones((), device="cuda")
+    with pytest.raises(RuntimeError, match="last dimension"):
+        M.layer_norm_forward(x)
+    with pytest.raises(RuntimeError, match="last dimension"):
+        M.layer_norm_backward(x, x, None, one, one)
