@@ -283,6 +283,9 @@ at::Tensor clip_grad_norm(at::TensorList grads, at::TensorList out, double max_n
     check_rc(morpho_sm100_clip_grad_norm(pairs.data(), n, static_cast<float>(max_norm), static_cast<float>(loss_scale),
                                          norm.data_ptr<float>(), ws.data_ptr(), bytes, stream_of(grads[0])),
              "clip_grad_norm");
+    // written through raw pointers: a graph that has saved one of them must notice
+    for (const at::Tensor& o : out)
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return norm;
 }
 

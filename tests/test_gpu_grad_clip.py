@@ -160,3 +160,19 @@ def test_refusals(cuda):
         M.clip_grad_norm([g[0].double()], 1.0)
     with pytest.raises(RuntimeError, match="CUDA"):
         M.clip_grad_norm(g, 1.0, out=[torch.empty(10)])
+
+
+def test_a_graph_that_saved_what_is_written_notices(cuda):
+    p = torch.nn.Parameter(torch.randn(100, device="cuda"))
+    p.grad = torch.randn(100, device="cuda")
+    x = torch.randn(100, device="cuda", requires_grad=True)
+    y = (x * p.grad).sum()
+    M.clip_grad_norm_([p], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out = torch.empty(100, device="cuda")
+    saved, read = out._version, p.grad._version
+    M.clip_grad_norm([p.grad], 0.1, out=[out])
+    assert out._version > saved and p.grad._version == read
+    with torch.inference_mode():
+        M.clip_grad_norm([torch.randn(100, device="cuda")], 0.1)
