@@ -334,7 +334,8 @@ extern "C" MORPHO_API int morpho_sm100_clip_grad_norm(const morpho_tensor_pair_t
     if (!(max_norm >= 0.0f)) return set_error(MORPHO_ERR_INVALID, "clip: max_norm must be non-negative (got %g)", static_cast<double>(max_norm));
     if (!(loss_scale > 0.0f) || loss_scale > 1e30f)
         return set_error(MORPHO_ERR_INVALID, "clip: loss_scale must be positive and finite (got %g)", static_cast<double>(loss_scale));
-    if (norm == nullptr) return set_error(MORPHO_ERR_INVALID, "clip: norm is NULL");
+    if (norm == nullptr || reinterpret_cast<uintptr_t>(norm) % sizeof(float) != 0)
+        return set_error(MORPHO_ERR_INVALID, "clip: norm is NULL or not 4-byte aligned");
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
         return set_error(MORPHO_ERR_INVALID, "clip: workspace is NULL or not 16-byte aligned");
     DeviceInfo dev;

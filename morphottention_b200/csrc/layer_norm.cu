@@ -928,11 +928,15 @@ int reduce_partials(const NormArgs& a, int n, void* dweight, void* dbias, cudaSt
     return MORPHO_OK;
 }
 
-int check_norm_ptr(const void* p, const char* name, int type) {
-    if (p == nullptr) return set_error(MORPHO_ERR_INVALID, "layer norm: %s is NULL", name);
+int check_norm_align(const void* p, const char* name, int type) {
     if (reinterpret_cast<uintptr_t>(p) % dtype_bytes(type) != 0)
         return set_error(MORPHO_ERR_INVALID, "layer norm: %s is not aligned to its element type", name);
     return MORPHO_OK;
+}
+
+int check_norm_ptr(const void* p, const char* name, int type) {
+    if (p == nullptr) return set_error(MORPHO_ERR_INVALID, "layer norm: %s is NULL", name);
+    return check_norm_align(p, name, type);
 }
 
 }  // namespace
@@ -953,6 +957,8 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_forward(const morpho_layer_nor
         MORPHO_TRY(check_norm_ptr(residual, "residual", p->type));
         MORPHO_TRY(check_norm_ptr(h, "h", p->type));
     }
+    MORPHO_TRY(check_norm_align(weight, "weight", p->weight_type));
+    MORPHO_TRY(check_norm_align(bias, "bias", p->weight_type));
     MORPHO_TRY(check_norm_ptr(mean, "mean", MORPHO_DTYPE_F32));
     MORPHO_TRY(check_norm_ptr(rstd, "rstd", MORPHO_DTYPE_F32));
     DeviceInfo dev;
@@ -995,6 +1001,8 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
     reset_launch_count();
     MORPHO_TRY(validate_norm(p));
     const bool sums = dweight != nullptr || dbias != nullptr;
+    MORPHO_TRY(check_norm_align(dweight, "dweight", p->weight_type));
+    MORPHO_TRY(check_norm_align(dbias, "dbias", p->weight_type));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p->rows == 0) {
         const size_t bytes = static_cast<size_t>(p->dim) * dtype_bytes(p->weight_type);
@@ -1005,6 +1013,7 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
     MORPHO_TRY(check_norm_ptr(grad_y, "grad_y", p->type));
     if (grad_h != nullptr) MORPHO_TRY(check_norm_ptr(grad_h, "grad_h", p->type));
     MORPHO_TRY(check_norm_ptr(h, "h", p->type));
+    MORPHO_TRY(check_norm_align(weight, "weight", p->weight_type));
     MORPHO_TRY(check_norm_ptr(mean, "mean", MORPHO_DTYPE_F32));
     MORPHO_TRY(check_norm_ptr(rstd, "rstd", MORPHO_DTYPE_F32));
     MORPHO_TRY(check_norm_ptr(dx, "dx", p->type));

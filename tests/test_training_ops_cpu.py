@@ -123,3 +123,28 @@ def test_backward_workspace_is_bounded():
     p = loss_problem(tokens=1 << 16, vocab=131072, dim=2048)
     n = L.morpho_sm100_linear_cross_entropy_backward_workspace_size(ctypes.byref(p))
     assert 0 < n < 2 * (1 << 16) * 131072 // 8
+
+
+def test_misaligned_parameters_refused():
+    """Pointers off their element's size, which a kernel would fault on, in every place that takes one."""
+    L, p = capi.lib(), norm_problem(weight_type=2)
+    at = [0x1000 * (i + 1) for i in range(9)]
+    names = ["x", "residual", "weight", "bias", "y", "h", "mean", "rstd"]
+    for i, name in enumerate(names):
+        bad = [a + (i == k) for k, a in enumerate(at[:8])]
+        assert L.morpho_sm100_layer_norm_forward(ctypes.byref(p), *bad, None) == capi.MORPHO_ERR_INVALID, name
+        assert f"{name} is not aligned" in capi.last_error()
+    assert L.morpho_sm100_layer_norm_forward(ctypes.byref(p), *at[:2], at[2] + 2, *at[3:8], None) == capi.MORPHO_ERR_INVALID
+    names = ["grad_y", "grad_h", "h", "weight", "mean", "rstd", "dx", "dweight", "dbias"]
+    for rows in (4, 0):
+        p = norm_problem(weight_type=2, rows=rows)
+        for i, name in enumerate(names):
+            if rows == 0 and not name.startswith(("dw", "db")):
+                continue
+            bad = [a + (i == k) for k, a in enumerate(at)]
+            rc = L.morpho_sm100_layer_norm_backward(ctypes.byref(p), *bad, 0xA0000, 1 << 30, None)
+            assert rc == capi.MORPHO_ERR_INVALID, name
+            assert f"{name} is not aligned" in capi.last_error()
+    pair = capi.MorphoTensorPair(0x1000, 0x1000, 8, 0, 0)
+    rc = L.morpho_sm100_clip_grad_norm(ctypes.byref(pair), 1, 1.0, 1.0, 0x8002, 0x10000, 1 << 20, None)
+    assert rc == capi.MORPHO_ERR_INVALID and "norm" in capi.last_error()
