@@ -4,8 +4,8 @@
 // Two passes over the gradients, bound by HBM: the first sums squares (fp32 within a thread, fp64
 // between threads, blocks and tensors, always in the same order), the second scales.  The norm is
 // needed before anything can be written, so the second pass reads the gradients again, from L2 for what
-// it still holds.  A norm that is not finite makes the gradients non-finite (0 * inf, NaN), as dividing
-// by it does.
+// it still holds.  An infinite gradient makes the norm infinite and the factor zero: finite gradients
+// become zero, infinite ones NaN (0 * inf); a NaN makes all of them NaN.
 //
 // The tensors are cut into chunks, dealt to a persistent grid, of one 2 KB segment for each warp.  The table
 // of tensors travels as a kernel parameter, so a launch needs no copy to the device and can be captured in a

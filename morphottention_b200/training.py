@@ -191,7 +191,8 @@ def clip_grad_norm(grads, max_norm: float, *, out=None, loss_scale: float = 1.0)
         16-bit gradients, say); None writes ``grads`` in place.
     :param loss_scale: the factor that the loss was multiplied by, removed here.
 
-    A norm that is infinite or NaN makes the results non-finite."""
+    An infinite gradient makes the norm infinite: finite gradients become zero, infinite ones NaN.  With
+    a NaN among them the norm and every result are NaN."""
     grads = list(grads)
     return _clip(grads, grads if out is None else list(out), max_norm, loss_scale)
 
