@@ -2,10 +2,11 @@
 //   norm = sqrt(sum_i |g_i|^2) / loss_scale,   c = min(1, max_norm / (norm + 1e-6)) / loss_scale
 //   out_i = c g_i
 // Two passes over the gradients, bound by HBM: the first sums squares (fp32 within a thread, fp64
-// between threads, blocks and tensors, always in the same order), the second scales.  The norm is
-// needed before anything can be written, so the second pass reads the gradients again, from L2 for what
-// it still holds.  An infinite gradient makes the norm infinite and the factor zero: finite gradients
-// become zero, infinite ones NaN (0 * inf); a NaN makes all of them NaN.
+// between threads, blocks and tensors, always in the same order; a thread whose fp32 sum leaves its range
+// takes its squares again in fp64), the second scales.  The norm is needed before anything can be written,
+// so the second pass reads the gradients again, from L2 for what it still holds.  An infinite gradient makes
+// the norm infinite and the factor zero: finite gradients become zero, infinite ones NaN (0 * inf); a NaN
+// makes all of them NaN.
 //
 // The tensors are cut into chunks, dealt to a persistent grid, of one 2 KB segment for each warp.  The table
 // of tensors travels as a kernel parameter, so a launch needs no copy to the device and can be captured in a
@@ -102,15 +103,44 @@ __device__ __forceinline__ void each_pack(const T* p, int n, int off, F f) {
     }
 }
 
+// A lane's fp32 sum of at most 32 squares is good between these: above, a square has overflowed; below, squares
+// under 2^-126 have lost bits that count.  (fp16's squares stay far inside.)
+constexpr float kLeastSum = 0x1p-100f, kMostSum = 0x1.fffffep127f;
+
 template <class T>
-__device__ __forceinline__ float segment_squares(const T* p, int n) {
+__device__ __noinline__ double segment_squares_wide(const T* p, int n) {
+    constexpr int V = 16 / sizeof(T);
+    double s = 0.0;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+#pragma unroll 1
+    for (int e = (threadIdx.x & 31) * V - off; e < n; e += 32 * V) {
+        const Pack<T, V> x = load_pack<T, V>(p + e);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const double d = to_f32(x.v[k]);
+            if (e + k >= 0 && e + k < n) s = fma(d, d, s);
+        }
+    }
+    return s;
+}
+
+// This lane's share of the sum of squares of the warp's n elements from p on.
+template <class T>
+__device__ __forceinline__ double segment_squares(const T* p, int n) {
     constexpr int V = 16 / sizeof(T);
     float s = 0.f;
+    uint32_t bits = 0u;  // of all elements: whether a sum of zero is one of zeros
     each_pack<V>(p, n, static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T)), [&](const auto& x, int e, auto whole) {
 #pragma unroll
         for (int k = 0; k < V; ++k)
             if (whole || (e + k >= 0 && e + k < n)) s = fmaf(to_f32(x.v[k]), to_f32(x.v[k]), s);
+        if (!std::is_same<T, __half>::value) {
+            const uint4 w = *reinterpret_cast<const uint4*>(x.v);
+            bits |= w.x | w.y | w.z | w.w;
+        }
     });
+    constexpr uint32_t magnitude = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;  // (zeros of either sign are zeros)
+    if (!std::is_same<T, __half>::value && (bits & magnitude) != 0u && !(s >= kLeastSum && s <= kMostSum)) return segment_squares_wide(p, n);
     return s;
 }
 

@@ -176,3 +176,17 @@ def test_a_graph_that_saved_what_is_written_notices(cuda):
     assert out._version > saved and p.grad._version == read
     with torch.inference_mode():
         M.clip_grad_norm([torch.randn(100, device="cuda")], 0.1)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", [1e20, 3e30, 1e-25, 1e-30])
+def test_squares_past_the_range_of_fp32(cuda, kind, size):
+    """Elements whose squares overflow or vanish in fp32 (the scale brings the results back to the size of one)."""
+    grads = [(g.float() * size).to(kind) for g in make([5, 8192 + 3, 40000, 33], [torch.float32])]
+    scale = min(size, 1e30)
+    check(grads, 0.5, float(torch.tensor(scale)), torch.float32)
+    # beside zeros, and as a few among smaller ones
+    for g in grads:
+        g[::3] = 0.0
+        g[1::7] *= 1e-6
+    check([*grads, torch.zeros(3000, device="cuda", dtype=kind)], 0.5, float(torch.tensor(scale)), torch.float32)
