@@ -322,6 +322,11 @@ MORPHO_API int morpho_sm100_device_status(void* stream, int reset, uint32_t* sta
  * the word with morpho_sm100_device_status. */
 MORPHO_API int morpho_sm100_selftest_wait_timeout(uint32_t limit_us, void* stream);
 
+/* The same for the layer norm's streamed rows: in one kernel of four groups of two warps, one warp of
+ * group 1 waits (1 s) for a row that is not fetched, which the status word records as kernel 7, site 2.
+ * seen (device, eight words): 1 for every warp that was told to go on, 0 for both of group 1. */
+MORPHO_API int morpho_sm100_selftest_row_wait(uint32_t* seen, void* stream);
+
 /* Design probe (no reference counterpart): the score the attention kernels issue as tcgen05
  * MMAs, computed instead on packed half2 CUDA-core math -- for every query row of every (batch,
  * head) the maximum over all keys of qc_i . k_j (cube_m/2 HFMA2 per pair, fp16 accumulation,

@@ -53,6 +53,7 @@ EXPORTED = (
     "morpho_sm100_device_status",
     "morpho_sm100_last_launch_count",
     "morpho_sm100_selftest_wait_timeout",
+    "morpho_sm100_selftest_row_wait",
     "morpho_sm100_profile_enable",
     "morpho_sm100_profile_collect",
     "morpho_sm100_profile_select",
@@ -157,6 +158,8 @@ def lib() -> ctypes.CDLL:
     L.morpho_sm100_last_launch_count.restype = i32
     L.morpho_sm100_selftest_wait_timeout.argtypes = [ctypes.c_uint32, vp]
     L.morpho_sm100_selftest_wait_timeout.restype = i32
+    L.morpho_sm100_selftest_row_wait.argtypes = [vp, vp]
+    L.morpho_sm100_selftest_row_wait.restype = i32
     L.morpho_sm100_profile_enable.argtypes = [i32]
     L.morpho_sm100_profile_enable.restype = None
     L.morpho_sm100_profile_select.argtypes = [ctypes.c_char_p]
@@ -494,3 +497,8 @@ def score_probe_half2(qc, kc, rowmax, stream=None) -> None:
 def selftest_wait_timeout(limit_us: int = 20000, stream=None) -> None:
     """Launch the failure-path self test (a bounded wait that is made to run out)."""
     _check(lib().morpho_sm100_selftest_wait_timeout(int(limit_us), _stream(stream)))
+
+
+def selftest_row_wait(seen, stream=None) -> None:
+    """Launch the self-test of a streamed row that never comes (``seen``: int32 [8] on the device)."""
+    _check(lib().morpho_sm100_selftest_row_wait(_ptr(seen), _stream(stream)))

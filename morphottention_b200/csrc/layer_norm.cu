@@ -461,9 +461,10 @@ constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = 32 * kStreamWarps;
 constexpr int kMaxStages = 8;
 
-// Sums of two values over the W warps of a group (threads 32 W of the CTA, group `g`).
+// Sums of two values over the W warps of a group (threads 32 W of the CTA, group `g`).  `ok`, which is uniform in
+// each warp, comes back as whether it holds in all of them: the group goes on or gives up as one.
 template <int W>
-__device__ __forceinline__ float2 warps_sum(float a, float b, float2 (*scratch)[kStreamWarps], int turn, int g) {
+__device__ __forceinline__ float2 warps_sum(float a, float b, bool& ok, float2 (*scratch)[kStreamWarps], int turn, int g) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, o);
@@ -472,7 +473,16 @@ __device__ __forceinline__ float2 warps_sum(float a, float b, float2 (*scratch)[
     if (W == 1) return make_float2(a, b);
     float2* s = scratch[turn & 1] + g * W;
     if ((threadIdx.x & 31) == 0) s[(threadIdx.x >> 5) & (W - 1)] = make_float2(a, b);
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(32 * W) : "memory");
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(ok)), "r"(1 + g), "n"(32 * W)
+        : "memory");
+    ok = all != 0u;
     float2 r = s[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) {
@@ -497,13 +507,15 @@ struct RowRing {
         bulk_load(dst + row_bytes, b, bytes, bar);
         if (c != nullptr) bulk_load(dst + 2 * row_bytes, c, bytes, bar);
     }
-    // After a wait for use i ran out: the copies that may still be in flight, each waited for in turn.
-    __device__ void drain(int i, uint32_t* status) const {
-        for (int k = 1; k < stages; ++k) mbar_wait(bars + 8 * ((i + k) % stages), ((i + k) / stages) & 1, status, K_NORM, 3);
+    // One thread, after the group gave up at use i: the n copies from there on that may still be in flight, each
+    // waited for in turn.
+    __device__ void drain(int i, int n, uint32_t* status) const {
+        for (int k = i; k < i + n; ++k) mbar_wait(bars + 8 * (k % stages), (k / stages) & 1, status, K_NORM, 3);
     }
     __device__ uint32_t stage(int i) const { return data + (i % stages) * stage_bytes; }
-    __device__ bool wait(int i, uint32_t* status, uint32_t site) const {
-        return mbar_wait(bars + 8 * (i % stages), (i / stages) & 1, status, K_NORM, site);
+    // A whole warp.
+    __device__ bool wait(int i, uint32_t* status) const {
+        return mbar_wait_warp(bars + 8 * (i % stages), (i / stages) & 1, status, K_NORM, 2);
     }
 };
 
@@ -583,10 +595,7 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
     for (int64_t row = first; row < a.rows; row += step, ++i) {
         const int64_t next = row + step < a.rows ? row + step : row;
         const float mu1 = a.mean[next], r1 = a.rstd[next];  // in flight beside this row
-        if (!ring.wait(i, a.status, 2)) {
-            ring.drain(i, a.status);
-            break;
-        }
+        bool ok = ring.wait(i, a.status);  // (if not, what follows up to the sums works on what lies there)
         const uint32_t src = ring.stage(i);
         float s0 = 0.f, s1 = 0.f;
         float xh[E], gw[E];
@@ -622,7 +631,13 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
                 }
             }
         }
-        const float2 s = warps_sum<W>(s0, s1, scratch, i, g);
+        const float2 s = warps_sum<W>(s0, s1, ok, scratch, i, g);
+        if (!ok) {
+            int fetched = 0;
+            while (fetched < a.stages && row + fetched * step < a.rows) ++fetched;
+            if (l == 0) ring.drain(i, fetched, a.status);
+            break;
+        }
         __syncwarp();
         if (l == 0) fetch(i + a.stages, row + a.stages * step);
         const float mg = s.x * inv, mgx = s.y * inv;
@@ -652,6 +667,20 @@ __global__ void __launch_bounds__(kStreamThreads, NV * 16 / sizeof(T) > 16 ? 1 :
     __syncthreads();  // over the rings: every fetched row has been waited for
     join_sums<VEC, NV, G, GROUPS>(reinterpret_cast<float*>(smem), dw, db, a.dim, a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.dim,
                                   [&](int i) { return SHIFT ? row_offset<VEC>(a, static_cast<int64_t>(blockIdx.x) * GROUPS + i) : 0; });
+}
+
+// Self-test of giving up: the second warp of group 1 waits for a row that is never fetched, the first did not have
+// to; seen[w]: what warp w was told (all groups but that one go on).
+__global__ void __launch_bounds__(kStreamThreads) row_wait_kernel(const NormArgs a, uint32_t* seen) {
+    constexpr int W = 2;
+    __shared__ __align__(128) uint8_t smem[16 * 2 * kStreamWarps / W];
+    __shared__ uint64_t bars[kStreamWarps / W * kMaxStages];
+    __shared__ float2 scratch[2][kStreamWarps];
+    const RowRing ring = make_ring<W>(smem, bars, a, 16, 2);
+    const int g = threadIdx.x / (32 * W), warp = threadIdx.x >> 5;
+    bool ok = g != 1 || warp % W == 0 || ring.wait(0, a.status);
+    const float2 s = warps_sum<W>(1.f, 2.f, ok, scratch, 0, g);
+    if ((threadIdx.x & 31) == 0) seen[warp] = ok && s.x == 32.f * W && s.y == 64.f * W;
 }
 
 // dweight / dbias = the sums of the `n` partial rows, in a fixed order: 32 columns per block, 32 threads a
@@ -1047,4 +1076,17 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_backward(const morpho_layer_no
         rc = backward_t<float>(dev, a, p->type, how, blocks, st);
     if (rc != MORPHO_OK || !sums) return rc;
     return reduce_partials(a, blocks, dweight, dbias, st);
+}
+
+extern "C" MORPHO_API int morpho_sm100_selftest_row_wait(uint32_t* seen, void* stream) {
+    clear_error();
+    MORPHO_TRY(check_norm_ptr(seen, "seen", MORPHO_DTYPE_F32));
+    DeviceInfo dev;
+    MORPHO_TRY(current_device_info(&dev));
+    NormArgs a{};
+    a.stages = 1;
+    a.status = dev.status;
+    row_wait_kernel<<<1, kStreamThreads, 0, static_cast<cudaStream_t>(stream)>>>(a, seen);
+    MORPHO_CUDA_TRY(cudaGetLastError());
+    return MORPHO_OK;
 }

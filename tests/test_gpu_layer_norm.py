@@ -4,10 +4,13 @@ Tolerances, per element: an output rounded to a type of unit roundoff u is off b
 value; everything before that rounding is fp32, whose error is a few 2^-24 of the terms that are added
 (ARITH bounds the count: sums over dim run as trees and short chains)."""
 
+import ctypes
+
 import pytest
 import torch
 
 import morphottention_b200 as M
+from morphottention_b200 import capi
 
 pytestmark = pytest.mark.gpu
 
@@ -341,3 +344,20 @@ def test_last_dimension_past_32_bits_is_refused(cuda):
         M.layer_norm_forward(x)
     with pytest.raises(RuntimeError, match="last dimension"):
         M.layer_norm_backward(x, x, None, one, one)
+
+
+def test_a_group_gives_up_as_one(cuda):
+    """One warp of a group waits for a row that never comes: the wait is bounded, both warps of the group
+    leave together (neither is left at the group's barrier) and the others go on."""
+    assert capi.device_status(reset=True) == 0
+    seen = torch.full((8,), -1, device="cuda", dtype=torch.int32)
+    capi.selftest_row_wait(seen)
+    assert seen.tolist() == [1, 1, 0, 0, 1, 1, 1, 1]
+    with pytest.raises(capi.MorphoError) as e:
+        capi.device_status(reset=False)
+    assert e.value.code == capi.MORPHO_ERR_TIMEOUT
+    word = ctypes.c_uint32(0)
+    capi.lib().morpho_sm100_device_status(torch.cuda.current_stream().cuda_stream, 1, ctypes.byref(word))
+    assert word.value == (0x80000000 | (2 << 8) | 7)
+    check(make(2400, 1032, torch.float16, torch.float16, residual=True))
+    assert capi.device_status(reset=True) == 0
