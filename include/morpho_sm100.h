@@ -283,6 +283,8 @@ MORPHO_API int morpho_sm100_linear_cross_entropy_forward(const morpho_vocab_loss
 /* dhidden [tokens, dim] and dweight [vocab, dim] (the inputs' type, contiguous, overwritten) for the
  * loss's gradient grad_loss: fp32 [tokens] (NONE) or one fp32.  The logits are computed again in pieces
  * of the vocabulary; the workspace holds two pieces of their gradient (each at most 512 MiB, or 256 columns).
+ * Tokens that are ignored, or whose gradient is zero (NONE), add nothing to either result, whatever their
+ * hidden rows hold.  lse is the forward's for these inputs.
  * Sums run in a fixed order: the same bits every run. */
 MORPHO_API size_t morpho_sm100_linear_cross_entropy_backward_workspace_size(const morpho_vocab_loss_t* p);
 MORPHO_API int morpho_sm100_linear_cross_entropy_backward(const morpho_vocab_loss_t* p, const float* grad_loss,

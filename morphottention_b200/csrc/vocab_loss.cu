@@ -93,6 +93,7 @@ struct alignas(64) Task {
     int K, k_blocks, kb_per_split;
     int items_end;  // work items of this task and those before it
     int v0, padded; // kDz: the piece's first column of the vocabulary; its width in whole panels
+    const uint8_t* dirty;  // per K block: whether B is read from Launch::clean instead (NULL: never)
 };
 
 // What the epilogues and the row kernels know of the rows.  A target that is neither in [0, V) nor
@@ -114,9 +115,24 @@ struct Rowwise {
     float* common;  // gmax / unit, the factor of the results; g_t = gmax r_t
 };
 
+// Rows that count for nothing (ignored, or of gradient zero) have zeros in dz, but dweight multiplies those by
+// hidden, and padding may hold NaN or infinities there.  Such a row shows in its lse.  The first launch of a
+// backward marks the blocks of BK rows that have one, and copies them with zeros in its place; dweight reads
+// the copies of marked blocks and hidden itself for all others.  (Backward, every block marked: 256 x 1000 x 256 22 -> 43 us,
+// 16384 x 1000 x 256 50 -> 77, 8192 x 32768 x 512 660 either way; none marked: 0.5 us at most.)
+struct Clean {
+    const uint16_t* hidden;
+    int64_t ld;
+    int D, blocks;
+    uint16_t* copy;  // [T][D]
+    uint8_t* dirty;  // [blocks]
+};
+
 constexpr int kMaxTasks = 3;
 struct Launch {
     Task task[kMaxTasks];
+    CUtensorMap clean;  // the copies
+    Clean cleaning;     // of the first launch
     int tasks;
     Rowwise rows;
     uint32_t* next;  // work items taken after the first of each pair; NULL: dealt round-robin
@@ -247,7 +263,7 @@ __device__ __forceinline__ void epi_dz(const Rowwise& p, const Task& t, uint32_t
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     x[i] = pack2<BF16>(u2f(q[2 * i]), u2f(q[2 * i + 1]));
-                    if (rt == 0.f) x[i] = 0u;  // an ignored row adds nothing, whatever its logits are
+                    if (rt == 0.f) x[i] = 0u;  // a row that counts for nothing adds nothing, whatever its logits are
                 }
                 stage_box(stage, lane, x);
                 if (lane == 0) {
@@ -394,6 +410,36 @@ __device__ __forceinline__ float largest_gradient(const Rowwise& p, float* scrat
     return most > 0.f ? fmaxf(most, p.unit * FLT_MIN) : 1.f;
 }
 
+// Marks block `b` of rows and copies it if need be: one warp.
+__device__ __forceinline__ void clean_block(const Rowwise& p, const Clean& c, int b, int lane) {
+    const int64_t row0 = static_cast<int64_t>(b) * BK;
+    uint32_t bad[BK / 32], any = 0u;
+#pragma unroll
+    for (int i = 0; i < BK / 32; ++i) {
+        const int64_t row = row0 + 32 * i + lane;
+        const bool out = row < p.T && !isfinite(p.lse[row]) &&
+                         (p.target[row] == p.ignore_index || (p.reduction == MORPHO_REDUCTION_NONE && p.grad[row] == 0.f));
+        bad[i] = __ballot_sync(0xffffffffu, out);
+        any |= bad[i];
+    }
+    if (lane == 0) c.dirty[b] = any != 0u;
+    if (any == 0u) return;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(BK), p.T - row0));
+#pragma unroll
+    for (int i = 0; i < BK / 32; ++i) {
+        const int last = min(32, rows - 32 * i);
+#pragma unroll 4
+        for (int r = 0; r < last; ++r) {
+            const int64_t row = row0 + 32 * i + r;
+            for (int col = lane * 8; col < c.D; col += 256) {
+                const uint4 x = *reinterpret_cast<const uint4*>(c.hidden + row * c.ld + col);
+                *reinterpret_cast<uint4*>(c.copy + row * c.D + col) = bad[i] >> r & 1u ? make_uint4(0u, 0u, 0u, 0u) : x;
+            }
+        }
+    }
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // the next launch reads it by TMA
+}
+
 // One operand of a stage: rows (M or N) x .. x + 127, K k .. k + 127, in two panels of 128 rows of 128 bytes.
 // K-major: the panels are the halves of K; MN-major: the halves of the rows, each with K down.
 __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap& map, uint32_t bar, bool mn, bool whole, int row0,
@@ -482,7 +528,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                 const Task& t = L.task[it.task];
                 const int kb0 = first_block(t, it), kb1 = end_block(t, it);
                 const int m = it.m0 + rank * kHalf, n = it.n0 + rank * kHalf;
+                uint32_t dirty = t.dirty != nullptr ? t.dirty[kb0] : 0u;
                 for (int kb = kb0; kb < kb1; ++kb, ++g) {
+                    const uint32_t dirty1 = t.dirty != nullptr && kb + 1 < kb1 ? t.dirty[kb + 1] : 0u;  // in flight beside this block
                     const int s = g % kStages;
                     if (g >= kStages && !mbar_wait(empty0 + 8 * s, ((g / kStages) & 1) ^ 1, L.status, K_VOCAB, 1)) {
                         *abort_flag = 1u;
@@ -492,7 +540,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                     const uint32_t fb = cluster_addr(full0 + 8 * s, 0);
                     if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * kStageBytes);
                     load_operand(sA, t.a, fb, t.a_mn, t.a_whole, t.a_row0, m, kb * BK);
-                    load_operand(sA + kOperandBytes, t.b, fb, t.b_mn, t.b_whole, t.b_row0, n, kb * BK);
+                    load_operand(sA + kOperandBytes, dirty ? L.clean : t.b, fb, t.b_mn, t.b_whole, t.b_row0, n, kb * BK);
+                    dirty = dirty1;
                 }
             }
             // No CTA leaves while commits to its barriers are on their way.
@@ -567,7 +616,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
             if (lane == 0) *L.rows.common = *L.rows.grad / (static_cast<float>(max(kept, int64_t(1))) * L.rows.unit);
         }
     } else if (warp == kEpiWarps + 2) {
-        // ---------------- scheduler, one thread of rank 0 ----------------
+        // ---------------- scheduler, one thread of rank 0 (and, in a backward's first launch, the rows that count for nothing) ----
+        if (L.rows.first)
+            for (int b = blockIdx.x; b < L.cleaning.blocks; b += gridDim.x) clean_block(L.rows, L.cleaning, b, lane);
         if (rank == 0 && lane == 0 && L.next != nullptr) {
             Item it = item_of(L, first);
             // the end is published twice: each epilogue set reads every other item
@@ -1009,6 +1060,9 @@ struct BwdPlan {
     uint16_t* dz[2];
     float *common, *hpart, *wpart;
     uint32_t* next;  // a work counter for each launch after the first
+    uint8_t* dirty;   // see Clean
+    uint16_t* clean;  // (NULL: dhidden, which is written last)
+    bool direct;      // dhidden is written by its product, not joined from partial sums
 };
 void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
     f->cut = cut_of(p, sms);
@@ -1017,8 +1071,11 @@ void plan_backward(Bump& b, const morpho_vocab_loss_t* p, int sms, BwdPlan* f) {
     for (int i = 0; i < 2; ++i) f->dz[i] = b.take<uint16_t>(i < c.pieces ? T * c.cols : 0);
     f->common = b.take<float>(1);
     f->next = b.take<uint32_t>(c.pieces);
-    f->hpart = b.take<float>(c.pieces > 1 || c.splits_h > 1 ? c.splits_h * T * D : 0);
+    f->direct = c.pieces == 1 && c.splits_h == 1;
+    f->hpart = b.take<float>(f->direct ? 0 : c.splits_h * T * D);
     f->wpart = b.take<float>(c.splits_w > 1 ? static_cast<size_t>(c.splits_w) * c.cols * D : 0);
+    f->dirty = b.take<uint8_t>(ceil_div(T, BK));
+    f->clean = f->direct ? b.take<uint16_t>(T * D) : nullptr;
 }
 
 int sm_count() {
@@ -1202,6 +1259,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
     r.common = f.common;
     const Cut& c = f.cut;
     const int64_t T = p->tokens, D = p->dim;
+    uint16_t* clean = f.clean != nullptr ? f.clean : static_cast<uint16_t*>(dhidden);
     auto width = [&](int i) { return std::min<int64_t>(c.cols, p->vocab - static_cast<int64_t>(i) * c.cols); };
     for (int i = -1; i < c.pieces; ++i) {
         Launch L{};
@@ -1222,15 +1280,16 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
             MORPHO_TRY(load_map(&h.a, &h.a_whole, f.dz[i & 1], T, padded, c.cols));
             MORPHO_TRY(load_map(&h.b, &h.b_whole, weight, p->vocab, D, ld_weight(p)));
             h.b_row0 = v0;
-            const bool direct = c.pieces == 1 && c.splits_h == 1;
-            if (direct)
+            w.dirty = f.dirty;
+            MORPHO_TRY(load_map(&L.clean, &w.b_whole, clean, T, D, D));
+            if (f.direct)
                 MORPHO_TRY(store_map(&h.out, dhidden, T, D, D));
             else
                 MORPHO_TRY(slab_map(&h.out, f.hpart, c.splits_h, T, D));
             // a shorter last piece may have fewer splits: the other slabs keep the earlier pieces' sums
             const int splits_h = static_cast<int>(std::min<int64_t>(c.splits_h, ceil_div(n, BK)));
             auto add_w = [&]() { return add_task(&L, w, c.splits_w > 1 ? kPart : kOut, true, true, n, D, T, c.splits_w); };
-            auto add_h = [&]() { return add_task(&L, h, direct ? kOut : i == 0 ? kPart : kPartAdd, false, true, T, D, n, splits_h); };
+            auto add_h = [&]() { return add_task(&L, h, f.direct ? kOut : i == 0 ? kPart : kPartAdd, false, true, T, D, n, splits_h); };
             // the longest items first: the pairs that finish early take the short ones (dz last)
             const bool h_first = ceil_div(n, splits_h) > ceil_div(T, c.splits_w);
             MORPHO_TRY(h_first ? add_h() : add_w());
@@ -1239,6 +1298,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
         } else {
             L.zero = f.next;
             L.zeros = c.pieces;
+            L.cleaning = Clean{static_cast<const uint16_t*>(hidden), ld_hidden(p), static_cast<int>(D), static_cast<int>(ceil_div(T, BK)), clean, f.dirty};
         }
         if (i + 1 < c.pieces) {
             Task z{};
@@ -1256,7 +1316,7 @@ int backward_t(const DeviceInfo& dev, const morpho_vocab_loss_t* p, const float*
             MORPHO_TRY(finish<BF16>(dev, f.wpart, c.splits_w, width(i) * D, f.common,
                                     static_cast<uint16_t*>(dweight) + static_cast<int64_t>(i) * c.cols * D, stream));
     }
-    if (c.pieces > 1 || c.splits_h > 1) MORPHO_TRY(finish<BF16>(dev, f.hpart, c.splits_h, T * D, f.common, dhidden, stream));
+    if (!f.direct) MORPHO_TRY(finish<BF16>(dev, f.hpart, c.splits_h, T * D, f.common, dhidden, stream));
     return MORPHO_OK;
 }
 

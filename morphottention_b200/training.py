@@ -149,7 +149,8 @@ def linear_cross_entropy_forward(hidden, weight, target, ignore_index: int = -10
 def linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index: int = -100,
                                   reduction: str = "mean"):
     """``[dhidden, dweight]`` for the loss's float32 gradient (``target``'s shape for ``"none"``, else one
-    element) and the forward's ``lse``.  Deterministic."""
+    element) and the forward's ``lse``.  Tokens that are ignored, or whose gradient is zero, add nothing to
+    either, whatever their hidden rows hold (NaN and infinities included).  Deterministic."""
     return _loss_backward(grad_loss, hidden, weight, target, lse, ignore_index,
                                              _reduction(reduction))
 

@@ -366,3 +366,46 @@ def test_refusals(cuda):
         M.linear_cross_entropy_backward(one, h, w, y, lse, IGNORE, "none")
     with pytest.raises(RuntimeError, match="lse must be"):
         M.linear_cross_entropy_backward(one, h, w, y, lse[:3])
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("T,V,D", [(1, 50, 64), (2, 300, 72), (20, 300, 64), (129, 777, 136), (1000, 300, 512), (5000, 3001, 128),
+                                   (300, 20000, 64), ((1 << 20) + 77, 300, 8)])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_rows_that_count_for_nothing_may_hold_anything(cuda, T, V, D, kind, reduction):
+    """Ignored rows with NaN and infinities give the same bits as zeros in their place, in dweight too (whose
+    product meets them): few and many tokens, one block of rows and many, split sums, two pieces of dz."""
+    g = torch.Generator(device="cuda").manual_seed(T + V + D)
+    h = torch.randn(T, D, generator=g, device="cuda").to(kind)
+    w = (torch.randn(V, D, generator=g, device="cuda") * D ** -0.5).to(kind)
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    grad = torch.rand(T, generator=g, device="cuda") + 0.5 if reduction == "none" else torch.ones((), device="cuda")
+    off = torch.rand(T, generator=g, device="cuda") < 0.2
+    off[256:640] = False  # blocks of rows without any
+    off[-1] = True
+    y[off] = IGNORE
+    if reduction == "none" and T > 2:  # a gradient of zero is as good
+        y[-1], grad[-1] = 0, 0.0
+    bad = torch.nonzero(off)[:, 0]
+    dirty, clean = h.clone(), h.clone()
+    for i, x in enumerate((float("nan"), float("inf"), -float("inf"))):
+        dirty[bad[i::3], (3 * i) % D] = x
+    dirty[-1] = float("nan")
+    clean[bad] = 0.0
+    got, want = [], []
+    for x, res in ((dirty, got), (clean, want)):
+        loss, lse = M.linear_cross_entropy_forward(x, w, y, IGNORE, reduction)
+        res += [loss[y != IGNORE][:-1] if reduction == "none" else loss,
+                *M.linear_cross_entropy_backward(grad, x, w, y, lse, IGNORE, reduction)]
+    assert capi.device_status(reset=True) == 0
+    for name, a, b in zip(("loss", "dhidden", "dweight"), got, want):
+        assert torch.isfinite(b).all() and torch.equal(a, b), name
+
+
+def test_non_finite_rows_that_count_are_seen(cuda):
+    h, w, y = make(300, 500, 64, torch.float16, ignored=0.2)
+    at = torch.nonzero(y != IGNORE)[7, 0]
+    h[at, 3] = float("nan")
+    _, lse = M.linear_cross_entropy_forward(h, w, y)
+    dh, dw = M.linear_cross_entropy_backward(torch.ones((), device="cuda"), h, w, y, lse)
+    assert dh[at].isnan().all() and dw.isnan().all()
