@@ -240,7 +240,8 @@ typedef struct morpho_layer_norm {
     int64_t stride_grad_h;
 } morpho_layer_norm_t;
 
-/* h is written only when residual is given (it may then be x's or residual's own buffer). */
+/* h is written only when residual is given (it may then be x's or residual's own buffer, if the rows of that
+ * one are contiguous; y overlaps no input). */
 MORPHO_API int morpho_sm100_layer_norm_forward(const morpho_layer_norm_t* p, const void* x, const void* residual,
                                                const void* weight, const void* bias, void* y, void* h, float* mean,
                                                float* rstd, void* stream);

@@ -985,6 +985,8 @@ extern "C" MORPHO_API int morpho_sm100_layer_norm_forward(const morpho_layer_nor
     if (residual != nullptr) {
         MORPHO_TRY(check_norm_ptr(residual, "residual", p->type));
         MORPHO_TRY(check_norm_ptr(h, "h", p->type));
+        const bool gaps = (h == x && p->stride_x != 0 && p->stride_x != p->dim) || (h == residual && p->stride_residual != 0 && p->stride_residual != p->dim);
+        if (gaps && p->rows > 1) return set_error(MORPHO_ERR_INVALID, "layer norm: h in place needs rows without gaps");
     }
     MORPHO_TRY(check_norm_align(weight, "weight", p->weight_type));
     MORPHO_TRY(check_norm_align(bias, "bias", p->weight_type));

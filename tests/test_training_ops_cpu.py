@@ -148,3 +148,13 @@ def test_misaligned_parameters_refused():
     pair = capi.MorphoTensorPair(0x1000, 0x1000, 8, 0, 0)
     rc = L.morpho_sm100_clip_grad_norm(ctypes.byref(pair), 1, 1.0, 1.0, 0x8002, 0x10000, 1 << 20, None)
     assert rc == capi.MORPHO_ERR_INVALID and "norm" in capi.last_error()
+
+
+def test_sum_in_place_of_strided_rows_refused():
+    """h is contiguous: written over rows with gaps it would overtake rows that are not read yet."""
+    L, at = capi.lib(), [0x1000 * (i + 1) for i in range(8)]
+    for strides, over in ((dict(stride_x=80), 0), (dict(stride_residual=72), 1)):
+        p = norm_problem(**strides)
+        args = [*at[:5], at[over], *at[6:]]
+        assert L.morpho_sm100_layer_norm_forward(ctypes.byref(p), *args, None) == capi.MORPHO_ERR_INVALID
+        assert "in place" in capi.last_error()
