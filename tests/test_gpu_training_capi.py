@@ -69,3 +69,17 @@ def test_clip_grad_norm(cuda):
     pair = capi.MorphoTensorPair(g[0].data_ptr(), out[0].data_ptr(), 5, 0, 2)
     rc = capi.lib().morpho_sm100_clip_grad_norm(ctypes.byref(pair), 1, 1.0, 1.0, norm.data_ptr(), out[2].data_ptr(), 8, None)
     assert rc == capi.MORPHO_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("rows,dim", [(700, 328), (3, 64), (5000, 777), (40, 33), (300, 9000)])
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_layer_norm_sum_in_place(cuda, rows, dim, over):
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    x, r = (torch.randn(rows, dim, generator=g, device=cuda, dtype=torch.float16) for _ in range(2))
+    w, b = torch.randn(dim, generator=g, device=cuda), torch.randn(dim, generator=g, device=cuda)
+    want = M.layer_norm_forward(x, w, b, 1e-5, r)
+    p = capi.layer_norm_problem(x, w)
+    y, mean, rstd = torch.empty_like(x), torch.empty(rows, device=cuda), torch.empty(rows, device=cuda)
+    h = x if over == "x" else r
+    capi.layer_norm_forward(p, x, r, w, b, y, h, mean, rstd)
+    assert all(torch.equal(a, c) for a, c in zip((y, mean, rstd, h), want))
