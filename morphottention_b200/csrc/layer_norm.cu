@@ -20,8 +20,9 @@
 // columns the rows in flight are bulk copies into a ring in shared memory instead (the streaming kernel).
 // Rows longer than a CTA's registers hold (dim > 8192) are read again from L2.
 //
-// Measured, with a residual, forward and backward: 65536 x 2048 bf16 372 us (5.8 TB/s, 89 % of a plain copy);
-// 12608 x 768 fp16 41.5 us (155 MB, 3.7 TB/s: launch, filling the ring and joining the sums are 9 us of it).
+// Measured, with a residual, forward and backward: 65536 x 2048 bf16 375 to 396 us on several B200s (5.4 to 5.7 TB/s, 83 to
+// 88 % of a plain copy); 12608 x 768 fp16 41 us (155 MB, 3.8 TB/s: launch, filling the ring and joining the sums are
+// 9 us of it).
 #include <algorithm>
 #include <initializer_list>
 

@@ -22,9 +22,11 @@
 // MMA issuer (rank 0 of the pair), warps 2-17 epilogue, warp 18 scheduler; the accumulator is double-buffered in TMEM, and
 // results leave through TMA stores from a swizzled box per warp.
 //
-// Measured, forward and backward (8TVD with the second logits): 8192 tokens, 32768 x 512 fp16 1.01 ms, 1.09 PFLOP/s;
-// 16384 tokens, 65536 x 1024 bf16 6.85 ms, 1.28 PFLOP/s, where the board's power limit holds a plain library product
-// at 1.39.  256 tokens, 1000 x 256: 34 us, its launches.  One token, 32768 x 1024, forward: 16.8 us, 67 MB read.
+// Measured, forward and backward (8TVD with the second logits; several B200s): 8192 tokens, 32768 x 512 fp16 1.02 to
+// 1.06 ms, 1.04 to 1.08 PFLOP/s; 16384 tokens, 65536 x 1024 bf16 6.85 to 7.15 ms, 1.23 to 1.28 PFLOP/s, where the board's
+// power limit holds a plain library product at 1.39.  256 tokens, 1000 x 256: 34 us, four dependent launches of 8 to 11,
+// most of it each one's own set-up (608 threads, cluster barriers, TMEM) and one tile's serial load, product and epilogue.
+// One token, 32768 x 1024, forward: 16.9 us, 67 MB read.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -66,7 +68,8 @@ enum Kind : int {
     kPartAdd // the same, added to what is there
 };
 
-// n / d for 0 <= n < 2^31 by one multiplication: mul = ceil(2^(32 + shift) / d), 2^shift the power of two not below d.
+// n / d for 0 <= n < 2^31 by one multiplication (Granlund and Montgomery, "Division by invariant integers using
+// multiplication"): mul is the low word of ceil(2^(32 + shift) / d), 2^shift the power of two not below d.
 struct FastDiv {
     uint32_t mul, shift, d;
     static FastDiv of(int d) {
@@ -605,7 +608,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1) voc
                 umma_commit_pair(acc_full0 + 8);
             }
         }
-        // One idle warp counts the rows of a mean for the launches that scale results by it.
+        // One warp counts the rows of a mean for the launches that scale results by it, beside the tiles.  With many
+        // tokens and a small vocabulary it takes longer than they do: backward of 2^20 tokens, 300 x 64, 2.97 ms where a
+        // sum takes 1.06; 16384 tokens, 1000 x 256, 51.5 us and 50.0; 8192, 32768 x 512, no difference.
         if (blockIdx.x == 1 && L.rows.first && L.rows.reduction != MORPHO_REDUCTION_NONE) {
             int64_t kept = 0;
             if (L.rows.reduction == MORPHO_REDUCTION_MEAN) {
@@ -955,8 +960,9 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const Rowwise 
 constexpr size_t kPieceBytes = 512u << 20;  // dz of one piece of the vocabulary, at most; two are held
 // Terms of one tensor-core sum, at most.  The tensor core truncates its fp32 accumulator at every
 // K = 16 step, which biases a long sum towards zero (2.3e-8 of it a step; 1.2 % measured after 2^23
-// terms), so longer sums are joined from sums of this length (5e-5, a fifth of fp16's own rounding) by
-// rounded fp32 additions.
+// terms), so longer sums are joined from sums of this length by rounded fp32 additions.  What that leaves in
+// dhidden and dweight, up to 5e-5 of a sum, is a tenth of the most that rounding the result to fp16 costs; the
+// logits, which are not rounded, are corrected instead (unbias_of).
 constexpr int kMaxK = 32768;
 constexpr int kMaxDim = 16384;
 
@@ -1209,7 +1215,9 @@ int launch_join(const Rowwise& r, const FwdPlan& f, float* loss, float* lse, cud
 // place of the running sum is lost, always towards zero.  For a sum that grows evenly to z in n steps these
 // units average 0.35 2^-23 z, so z comes out short by n 2.1e-8 of itself (measured 1.5e-8 in bf16, where
 // early sums are exact, and 1.9e-8 in fp16); 1.8e-8 is put back.  At dim 1024 that takes the error of a
-// target's logit from 8e-6 to that of an fp32 sum, 3e-6.
+// target's logit from 8e-6 to that of an fp32 sum, 3e-6.  The constant is fitted to sums whose terms are alike.  Where
+// nothing is truncated (a hidden row with a few non-zero elements) it is itself the error: 1.2e-6 of the logit
+// at dim 1024, 1.8e-5 at 16384, which is what the other sums would be short by without it.
 float unbias_of(int dim) { return static_cast<float>(1.0 + (dim + 15) / 16 * 1.8e-8); }
 
 Rowwise rows_of(const morpho_vocab_loss_t* p, const int64_t* target) {
